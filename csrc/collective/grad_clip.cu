@@ -1,0 +1,302 @@
+// Global gradient norm over many tensors, and clipping.
+//
+//   s = sum_i sum_j g_ij^2,  norm = sqrt(s),  out_ij = g_ij * min(1, max_norm / (norm + 1e-6))
+//
+// Both passes are bound by memory: the norm reads every gradient once, the scaling reads it again
+// and writes it.  The tensors are cut into chunks of 4096 elements, counted through all tensors, and
+// every block takes an equal, contiguous run of chunks, so a list of hundreds of small tensors and
+// one of a few huge ones load the GPU alike, in one launch.  The sums depend on nothing but the
+// plan and the grid: no atomics.
+//
+// Squares of 8 neighbours are summed in fp32 (an error of a few 2^-24) and those sums in fp64, so
+// the length of the list costs no precision.  A group whose fp32 sum leaves the range in which that
+// holds (overflow, or squares near fp32's smallest numbers) is summed again in fp64.
+#include "collective/operators.hpp"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+namespace ugdr::coll {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kGroup = 8;    // elements a thread takes at once: 16 or 32 bytes
+constexpr int kUnroll = 4;   // groups in flight per thread
+static_assert(kThreads * kGroup == kGradChunk, "one group per thread and chunk");
+
+template <int TYPE> struct Element;
+template <> struct Element<UGDR_X_TYPE_BF16> {
+    using type = __nv_bfloat16;
+};
+template <> struct Element<UGDR_X_TYPE_FP16> {
+    using type = __half;
+};
+template <> struct Element<UGDR_X_TYPE_FP32> {
+    using type = float;
+};
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void from_float(float &d, float v) { d = v; }
+__device__ __forceinline__ void from_float(__half &d, float v) { d = __float2half_rn(v); }
+__device__ __forceinline__ void from_float(__nv_bfloat16 &d, float v) { d = __float2bfloat16_rn(v); }
+
+template <typename T> struct alignas(sizeof(T) * kGroup) Group {
+    T v[kGroup];
+};
+
+template <typename T> __device__ __forceinline__ Group<T> load_group(const T *p) {
+    Group<T> g;
+    if constexpr (sizeof(T) == 4) {
+        uint32_t *w = reinterpret_cast<uint32_t *>(g.v);
+        asm volatile("ld.global.v8.u32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                     : "l"(p)
+                     : "memory");
+    } else {
+        uint32_t *w = reinterpret_cast<uint32_t *>(g.v);
+        asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "l"(p)
+                     : "memory");
+    }
+    return g;
+}
+template <typename T> __device__ __forceinline__ void store_group(T *p, const Group<T> &g) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(g.v);
+    if constexpr (sizeof(T) == 4)
+        asm volatile("st.global.v8.u32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                     "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                     : "memory");
+    else
+        asm volatile("st.global.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                     : "memory");
+}
+
+// The tensor list of a plan: the tensors and the chunk that each begins with.
+struct Plan {
+    const ugdr_x_grad *grads;
+    const uint32_t *first;
+    int n;
+};
+
+// The tensor that holds `chunk`: every thread looks at some of them, one finds it.
+__device__ int tensor_of(const Plan &p, uint32_t chunk) {
+    __shared__ int found;
+    for (int i = threadIdx.x; i < p.n; i += kThreads)
+        if (p.first[i] <= chunk && chunk < p.first[i + 1]) found = i;
+    __syncthreads();
+    const int i = found;
+    __syncthreads();
+    return i;
+}
+
+__device__ double block_sum(double v) {
+    __shared__ double warp_sums[kThreads / 32];
+    for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (threadIdx.x % 32 == 0) warp_sums[threadIdx.x / 32] = v;
+    __syncthreads();
+    v = 0;
+    for (int w = 0; w < kThreads / 32; ++w) v += warp_sums[w];
+    return v;
+}
+
+__device__ __forceinline__ double squares(const float (&f)[kGroup]) {
+    float s = 0.f, most = 0.f;
+#pragma unroll
+    for (int j = 0; j < kGroup; ++j) {
+        s = fmaf(f[j], f[j], s);
+        most = fmaxf(most, fabsf(f[j]));
+    }
+    if (s < 3e38f && (s > 1e-30f || most == 0.f)) return s;
+    double d = 0;
+#pragma unroll
+    for (int j = 0; j < kGroup; ++j) d = fma(double(f[j]), double(f[j]), d);
+    return d;
+}
+
+// Elements before the tensor's first that make its base a multiple of a group's bytes: chunk c
+// holds the elements [4096 c - lead, 4096 (c + 1) - lead) that exist, so that every whole group is
+// one aligned load whatever the tensor's own alignment.
+template <typename T> __device__ __forceinline__ uint32_t lead_of(const T *p) {
+    return uint32_t(reinterpret_cast<uintptr_t>(p) % (sizeof(T) * kGroup) / sizeof(T));
+}
+
+// The squares of the chunks [c0, c1) of one tensor.
+template <int TYPE> __device__ double span_squares(const ugdr_x_grad &t, uint32_t c0, uint32_t c1) {
+    using T = typename Element<TYPE>::type;
+    const T *g = static_cast<const T *>(t.grad);
+    const int64_t lead = lead_of(g), n = int64_t(t.count);
+    double acc = 0;
+    for (uint32_t c = c0; c < c1; c += kUnroll) {
+        Group<T> v[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int64_t at = int64_t(c + u) * kGradChunk + threadIdx.x * kGroup - lead;
+            if (c + u < c1 && at >= 0 && at + kGroup <= n) {
+                v[u] = load_group(g + at);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kGroup; ++j) {
+                    from_float(v[u].v[j], 0.f);
+                    if (c + u < c1 && at + j >= 0 && at + j < n) v[u].v[j] = g[at + j];
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            float f[kGroup];
+#pragma unroll
+            for (int j = 0; j < kGroup; ++j) f[j] = to_float(v[u].v[j]);
+            acc += squares(f);
+        }
+    }
+    return acc;
+}
+
+__device__ __forceinline__ uint32_t share(uint32_t chunks, uint32_t block) {
+    return uint32_t(uint64_t(chunks) * block / gridDim.x);
+}
+
+__global__ void __launch_bounds__(kThreads, 2) grad_norm_kernel(Plan p, uint32_t chunks, double *partials) {
+    const uint32_t c1 = share(chunks, blockIdx.x + 1);
+    uint32_t c = share(chunks, blockIdx.x);
+    double acc = 0;
+    if (c < c1) {
+        for (int i = tensor_of(p, c); c < c1; ++i) {
+            const ugdr_x_grad t = p.grads[i];
+            const uint32_t first = p.first[i], end = min(p.first[i + 1], c1);
+            if (c >= end) continue;  // a tensor without elements
+            if (t.grad_type == UGDR_X_TYPE_BF16)
+                acc += span_squares<UGDR_X_TYPE_BF16>(t, c - first, end - first);
+            else if (t.grad_type == UGDR_X_TYPE_FP16)
+                acc += span_squares<UGDR_X_TYPE_FP16>(t, c - first, end - first);
+            else
+                acc += span_squares<UGDR_X_TYPE_FP32>(t, c - first, end - first);
+            c = end;
+        }
+    }
+    acc = block_sum(acc);
+    if (threadIdx.x == 0) partials[blockIdx.x] = acc;
+}
+
+__device__ double partial_sum(const double *partials, int n) {
+    double v = 0;
+    for (int i = threadIdx.x; i < n; i += kThreads) v += partials[i];
+    return block_sum(v);
+}
+
+__global__ void __launch_bounds__(kThreads) grad_sum_kernel(const double *partials, int n, double *sum_squares) {
+    const double s = partial_sum(partials, n);
+    if (threadIdx.x == 0) *sum_squares = s;
+}
+
+// The chunks [c0, c1) of one tensor scaled, the last ones first.
+template <int IN, int OUT> __device__ void span_scale(const ugdr_x_grad &t, uint32_t c0, uint32_t c1, float coef) {
+    using T = typename Element<IN>::type;
+    using O = typename Element<OUT>::type;
+    const T *g = static_cast<const T *>(t.grad);
+    O *out = static_cast<O *>(t.out);
+    const int64_t lead = lead_of(g), n = int64_t(t.count);
+    const bool whole = lead_of(out) == uint32_t(lead);  // whole groups of the output are aligned too
+    for (uint32_t left = c1 - c0; left > 0; left -= min(left, uint32_t(kUnroll))) {
+        Group<T> v[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int64_t at = (int64_t(c0) + left - 1 - u) * kGradChunk + threadIdx.x * kGroup - lead;
+            if (uint32_t(u) < left && at >= 0 && at + kGroup <= n) v[u] = load_group(g + at);
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            if (uint32_t(u) >= left) break;
+            const int64_t at = (int64_t(c0) + left - 1 - u) * kGradChunk + threadIdx.x * kGroup - lead;
+            if (at >= 0 && at + kGroup <= n) {
+                Group<O> o;
+#pragma unroll
+                for (int j = 0; j < kGroup; ++j) from_float(o.v[j], to_float(v[u].v[j]) * coef);
+                if (whole) {
+                    store_group(out + at, o);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kGroup; ++j) out[at + j] = o.v[j];
+                }
+            } else {
+                for (int j = 0; j < kGroup; ++j)
+                    if (at + j >= 0 && at + j < n) from_float(out[at + j], to_float(g[at + j]) * coef);
+            }
+        }
+    }
+}
+
+// Every block sums the partial sums itself, in one order, so no block waits for another; then it
+// scales its run of chunks backwards: what the norm pass read last is what the L2 still holds.
+__global__ void __launch_bounds__(kThreads, 2) grad_scale_kernel(Plan p, uint32_t chunks, const double *partials,
+                                                                 int npartials, float max_norm, float *norm_out) {
+    const double norm = sqrt(partial_sum(partials, npartials));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = float(norm);
+    const double ratio = double(max_norm) / (norm + 1e-6);
+    const float coef = ratio > 1.0 ? 1.f : float(ratio);  // a NaN stays one
+    const uint32_t c0 = share(chunks, blockIdx.x);
+    uint32_t c = share(chunks, blockIdx.x + 1);
+    if (c0 >= c) return;
+    for (int i = tensor_of(p, c - 1); c > c0; --i) {
+        const ugdr_x_grad t = p.grads[i];
+        const uint32_t first = p.first[i], from = max(first, c0);
+        if (from >= c) continue;
+        const uint32_t a = from - first, b = c - first;
+        c = from;
+        if (coef == 1.f && t.out == t.grad && t.out_type == t.grad_type) continue;
+        if (t.grad_type == UGDR_X_TYPE_BF16) {
+            if (t.out_type == UGDR_X_TYPE_BF16)
+                span_scale<UGDR_X_TYPE_BF16, UGDR_X_TYPE_BF16>(t, a, b, coef);
+            else
+                span_scale<UGDR_X_TYPE_BF16, UGDR_X_TYPE_FP32>(t, a, b, coef);
+        } else if (t.grad_type == UGDR_X_TYPE_FP16) {
+            if (t.out_type == UGDR_X_TYPE_FP16)
+                span_scale<UGDR_X_TYPE_FP16, UGDR_X_TYPE_FP16>(t, a, b, coef);
+            else
+                span_scale<UGDR_X_TYPE_FP16, UGDR_X_TYPE_FP32>(t, a, b, coef);
+        } else {
+            span_scale<UGDR_X_TYPE_FP32, UGDR_X_TYPE_FP32>(t, a, b, coef);
+        }
+    }
+}
+
+Plan as_plan(const void *plan, int n) {
+    const auto *grads = static_cast<const ugdr_x_grad *>(plan);
+    return {grads, reinterpret_cast<const uint32_t *>(grads + n), n};
+}
+
+// Two blocks per SM, fewer when there are fewer chunks; at least one, which writes the sum or norm.
+int blocks_for(uint64_t chunks) {
+    int device = 0, sms = 148;
+    cudaGetDevice(&device);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    const uint64_t most = uint64_t(sms) * 2 < UGDR_X_GRAD_PARTIALS ? uint64_t(sms) * 2 : UGDR_X_GRAD_PARTIALS;
+    return int(chunks < 1 ? 1 : chunks < most ? chunks : most);
+}
+
+}  // namespace
+
+int launch_grad_sum_squares(const void *plan, int n, uint64_t chunks, double *partials, double *sum_squares,
+                            cudaStream_t s) {
+    const int blocks = blocks_for(chunks);
+    grad_norm_kernel<<<blocks, kThreads, 0, s>>>(as_plan(plan, n), uint32_t(chunks), partials);
+    grad_sum_kernel<<<1, kThreads, 0, s>>>(partials, blocks, sum_squares);
+    return int(cudaGetLastError());
+}
+
+int launch_grad_clip(const void *plan, int n, uint64_t chunks, double *partials, const double *sum_squares,
+                     float max_norm, float *norm_out, cudaStream_t s) {
+    const int blocks = blocks_for(chunks);
+    if (sum_squares == nullptr)
+        grad_norm_kernel<<<blocks, kThreads, 0, s>>>(as_plan(plan, n), uint32_t(chunks), partials);
+    grad_scale_kernel<<<blocks, kThreads, 0, s>>>(as_plan(plan, n), uint32_t(chunks),
+                                                  sum_squares == nullptr ? partials : sum_squares,
+                                                  sum_squares == nullptr ? blocks : 1, max_norm, norm_out);
+    return int(cudaGetLastError());
+}
+
+}  // namespace ugdr::coll

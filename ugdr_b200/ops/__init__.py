@@ -5,6 +5,10 @@
 * bulk_copy_ms(dst, src)   the same copy staged through shared memory by the TMA bulk engine
 * moe_route(ids, nexp)     deterministic counting sort of (token, k) rows by expert
 * register(pd, tensor)     a verbs MR over a tensor's bytes (local write + remote read / write)
+* expert_ffn(...), expert_ffn_train(...), expert_ffn_backward(...)   the experts' gated
+                           feed-forward block on rows grouped by expert (ops/experts.py)
+* GradClip(grads)          the global gradient norm over many tensors, and clipping (ops/grads.py)
+* check_status()           raises for faults that the expert kernels recorded on the device
 * kernel_attributes()      registers, spills, static shared memory and blocks per SM of every
                            kernel of the library on the current device
 
@@ -18,6 +22,9 @@ import torch
 
 from .. import _native as N
 from ..parallel.collectives import moe_route  # noqa: F401  (re-exported)
+from .experts import (ExpertFFNSaved, check_status, expert_ffn, expert_ffn_backward,  # noqa: F401
+                      expert_ffn_train)
+from .grads import GradClip  # noqa: F401
 
 
 class KernelAttr(C.Structure):

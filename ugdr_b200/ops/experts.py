@@ -1,0 +1,213 @@
+"""The experts' gated feed-forward block on rows grouped by expert, as the MoE dispatch leaves them
+in the receive area (`MoEAllToAll.recv_view()` with `MoEAllToAll.expert_rows()`):
+
+    h = act(x Wg^T) * (x Wu^T),   y = h Wo^T
+
+with every row's own expert's weights.  Serving calls `expert_ffn`; a training step calls
+`expert_ffn_train`, which keeps what the backward pass needs, and `expert_ffn_backward`.
+
+Tensors are contiguous CUDA tensors on one device, bfloat16 or float16 throughout (products and
+sums in fp32):
+
+    x, y, dy, dx   [rows, hidden]             hidden and inner multiples of 8
+    counts         [experts] int32            rows of each expert, in order; read on the device
+    w_in           [experts, 2, inner, hidden]  the gate's, then the up projection's weights
+    w_out          [experts, hidden, inner]
+
+Rows behind the last group (the unused end of a receive area) are left as they were.  Calls are
+enqueued on `stream` (default: the device's current stream), whose order the inputs must respect,
+and may be captured into a CUDA graph.  They do not take part in autograd.  Counts that are
+negative or add up to more than `rows` are recorded on the device: `check_status()` raises for
+them, as it does when a bounded wait inside a kernel ran out.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+from typing import NamedTuple
+
+import torch
+
+from .. import _native as N
+from ..parallel.peers import check
+
+_TYPES = {torch.bfloat16: 0, torch.float16: 1}
+_ACTS = {"silu": 0, "gelu": 1}
+MAX_EXPERTS = 4096
+
+
+class _Experts(C.Structure):
+    _fields_ = [("counts", C.c_void_p), ("w_in", C.c_void_p), ("w_out", C.c_void_p), ("status", C.c_void_p),
+                ("rows", C.c_uint64), ("nexp", C.c_int), ("hidden", C.c_int), ("inner", C.c_int),
+                ("type", C.c_int), ("act", C.c_int)]
+
+
+class ExpertFFNSaved(NamedTuple):
+    """What a training forward pass keeps for `expert_ffn_backward` (2 * 3 * rows * inner bytes)."""
+
+    h: torch.Tensor   # [rows, inner]
+    gu: torch.Tensor  # [rows, 2, inner]
+
+
+_status: dict[int, torch.Tensor] = {}
+
+
+def _lib() -> C.CDLL:
+    L = N.lib()
+    if not getattr(L, "_expert_sigs", False):
+        vp = C.c_void_p
+        L.ugdr_x_expert_ffn.restype = C.c_int
+        L.ugdr_x_expert_ffn.argtypes = [C.POINTER(_Experts)] + [vp] * 5
+        L.ugdr_x_expert_ffn_backward.restype = C.c_int
+        L.ugdr_x_expert_ffn_backward.argtypes = [C.POINTER(_Experts)] + [vp] * 9
+        L._expert_sigs = True
+    return L
+
+
+@contextlib.contextmanager
+def _on(device: torch.device, stream: torch.cuda.Stream | None):
+    """The tensors' device current, and `stream` the one that outputs and scratch are allocated for."""
+    if stream is not None and stream.device != device:
+        raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+    with torch.cuda.device(device):
+        if stream is None:
+            yield torch.cuda.current_stream(device).cuda_stream
+        else:
+            with torch.cuda.stream(stream):
+                yield stream.cuda_stream
+
+
+def _status_word(device: torch.device) -> torch.Tensor:
+    word = _status.get(device.index)
+    if word is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("call an expert operator once on this device before capturing it into a graph")
+        word = _status[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+        torch.cuda.current_stream(device).synchronize()  # zero before any stream may write it
+    return word
+
+
+def check_status(device: torch.device | int | None = None) -> None:
+    """Wait for `device` (default: the current one) and raise RuntimeError if an expert operator on
+    it recorded a fault since the last check."""
+    index = device if isinstance(device, int) else torch.device(device or "cuda").index
+    word = _status.get(torch.cuda.current_device() if index is None else index)
+    if word is None:
+        return
+    torch.cuda.synchronize(word.device)
+    st = int(word.item())
+    if st:
+        word.zero_()
+        raise RuntimeError({1: "a bounded wait inside an expert kernel ran out",
+                            2: "expert counts are negative or exceed the rows"}.get(st, f"status {st}"))
+
+
+def _rows(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor) -> None:
+    if not isinstance(t, torch.Tensor) or t.device != like.device or t.dtype != like.dtype:
+        raise ValueError(f"{name} must be a {like.dtype} tensor on {like.device}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+    if not t.is_contiguous() or t.data_ptr() % 16:
+        raise ValueError(f"{name} must be contiguous and 16-byte aligned")
+
+
+def _checked(x, counts, w_in, w_out, act: str) -> _Experts:
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _TYPES or x.dim() != 2:
+        raise ValueError("x must be a CUDA tensor [rows, hidden] of bfloat16 or float16")
+    if act not in _ACTS:
+        raise ValueError(f"act must be one of {sorted(_ACTS)}, got {act!r}")
+    rows, hidden = x.shape
+    if not isinstance(counts, torch.Tensor) or counts.dtype != torch.int32 or counts.dim() != 1 \
+            or counts.device != x.device or not counts.is_contiguous():
+        raise ValueError(f"counts must be a contiguous int32 tensor [experts] on {x.device}")
+    nexp = counts.numel()
+    if not 1 <= nexp <= MAX_EXPERTS:
+        raise ValueError(f"1..{MAX_EXPERTS} experts supported, got {nexp}")
+    if not isinstance(w_out, torch.Tensor) or w_out.dim() != 3:
+        raise ValueError("w_out must be a tensor [experts, hidden, inner]")
+    inner = w_out.shape[2]
+    if hidden < 8 or hidden % 8 or inner < 8 or inner % 8:
+        raise ValueError(f"hidden and inner must be multiples of 8, got {hidden} and {inner}")
+    if rows >= 1 << 31:
+        raise ValueError(f"at most 2**31 - 1 rows, got {rows}")
+    _rows(x, "x", (rows, hidden), x)
+    _rows(w_in, "w_in", (nexp, 2, inner, hidden), x)
+    _rows(w_out, "w_out", (nexp, hidden, inner), x)
+    return _Experts(counts.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), None, rows, nexp, hidden, inner,
+                    _TYPES[x.dtype], _ACTS[act])
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    return a0 < b0 + b.numel() * b.element_size() and b0 < a0 + a.numel() * a.element_size()
+
+
+def _apart(out: torch.Tensor, name: str, inputs: dict, same: tuple = ()) -> None:
+    """`out` overlaps none of the inputs; those named in `same` it may be as a whole."""
+    for other, t in inputs.items():
+        if _overlap(out, t) and not (other in same and out.data_ptr() == t.data_ptr()):
+            raise ValueError(f"{name} must not overlap {other}" + (" unless it is the same tensor" if other in same
+                                                                    else ""))
+
+
+def _forward(x, counts, w_in, w_out, act, out, stream, train):
+    m = _checked(x, counts, w_in, w_out, act)
+    if out is not None:
+        _rows(out, "out", tuple(x.shape), x)
+        _apart(out, "out", {"x": x, "counts": counts, "w_in": w_in, "w_out": w_out}, () if train else ("x",))
+    with _on(x.device, stream) as s:
+        word = _status_word(x.device)
+        y = torch.empty_like(x) if out is None else out
+        h = torch.empty(m.rows, m.inner, dtype=x.dtype, device=x.device)
+        gu = torch.empty(m.rows, 2, m.inner, dtype=x.dtype, device=x.device) if train else None
+        m.status = word.data_ptr()
+        check(_lib().ugdr_x_expert_ffn(C.byref(m), x.data_ptr(), y.data_ptr(), h.data_ptr(),
+                                       gu.data_ptr() if train else None, s), "ugdr_x_expert_ffn")
+    return y, ExpertFFNSaved(h, gu) if train else None
+
+
+def expert_ffn(x: torch.Tensor, counts: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, act: str = "silu",
+               out: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """y [rows, hidden] of the block, into `out` if given (which may be `x` itself: the experts in
+    place in the receive area).  act: "silu" or "gelu" (the exact one)."""
+    return _forward(x, counts, w_in, w_out, act, out, stream, False)[0]
+
+
+def expert_ffn_train(x: torch.Tensor, counts: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
+                     act: str = "silu", out: torch.Tensor | None = None,
+                     stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, ExpertFFNSaved]:
+    """(y, saved): as expert_ffn, keeping what expert_ffn_backward needs beside x, which has to
+    stay as it is until then (`out` must not overlap it)."""
+    return _forward(x, counts, w_in, w_out, act, out, stream, True)
+
+
+def expert_ffn_backward(dy: torch.Tensor, x: torch.Tensor, counts: torch.Tensor, w_in: torch.Tensor,
+                        w_out: torch.Tensor, saved: ExpertFFNSaved, act: str = "silu",
+                        dx: torch.Tensor | None = None, dw_in: torch.Tensor | None = None,
+                        dw_out: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None
+                        ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dw_in, dw_out) from dy = d loss / d y and the forward pass's inputs, into the tensors
+    given for them.  dx may be dy or x itself.  Weight gradients of experts without rows are
+    zeros."""
+    m = _checked(x, counts, w_in, w_out, act)
+    _rows(dy, "dy", tuple(x.shape), x)
+    _rows(saved.h, "saved.h", (m.rows, m.inner), x)
+    _rows(saved.gu, "saved.gu", (m.rows, 2, m.inner), x)
+    inputs = {"dy": dy, "x": x, "counts": counts, "w_in": w_in, "w_out": w_out, "saved.h": saved.h,
+              "saved.gu": saved.gu}
+    for name, t, like in (("dx", dx, x), ("dw_in", dw_in, w_in), ("dw_out", dw_out, w_out)):
+        if t is not None:
+            _rows(t, name, tuple(like.shape), x)
+            _apart(t, name, inputs, ("dy", "x") if name == "dx" else ())
+            inputs[name] = t
+    with _on(x.device, stream) as s:
+        word = _status_word(x.device)
+        dx = torch.empty_like(x) if dx is None else dx
+        dw_in = torch.empty_like(w_in) if dw_in is None else dw_in
+        dw_out = torch.empty_like(w_out) if dw_out is None else dw_out
+        dgu = torch.empty(m.rows, 2, m.inner, dtype=x.dtype, device=x.device)
+        m.status = word.data_ptr()
+        check(_lib().ugdr_x_expert_ffn_backward(C.byref(m), dy.data_ptr(), x.data_ptr(), saved.h.data_ptr(),
+                                                saved.gu.data_ptr(), dgu.data_ptr(), dx.data_ptr(),
+                                                dw_in.data_ptr(), dw_out.data_ptr(), s), "ugdr_x_expert_ffn_backward")
+    return dx, dw_in, dw_out

@@ -71,6 +71,14 @@ class MoEAllToAll:
         return self.g.view(torch.bfloat16, self.recv_rows * self.hidden, self.recv_off).view(self.recv_rows,
                                                                                              self.hidden)
 
+    def expert_rows(self) -> torch.Tensor:
+        """Rows that the last dispatch brought for each of this rank's experts, [experts per rank]
+        int32 on the device, in the order of their groups in `recv_view()`: the counts that
+        `ugdr_b200.ops.expert_ffn` takes.  On the current stream, between dispatch and combine."""
+        table = self.g.view(torch.int32, self.g.world * self.nexp, self.table_off).view(self.g.world, self.nexp)
+        mine = slice(self.g.rank * self.exp_per_rank, (self.g.rank + 1) * self.exp_per_rank)
+        return table[:, mine].sum(0, dtype=torch.int32)
+
     def dispatch(self, x: torch.Tensor, expert_ids: torch.Tensor, ctas: int = 0,
                  stream: torch.cuda.Stream | None = None) -> None:
         assert x.dtype == torch.bfloat16 and x.is_contiguous() and x.shape == (self.tokens, self.hidden)
