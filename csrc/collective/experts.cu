@@ -4,22 +4,333 @@
 //   dh = dy Wo, dg = dh * u * a'(g), du = dh * a(g), dx = dg Wg + du Wu
 //   dWg = dg^T x, dWu = du^T x, dWo = dy^T h
 //
-// Plain tiled kernels: one 64 x 64 tile of a product per block, fp32 accumulation.
+// Six grouped matrix products, one persistent kernel template: with some hundred rows per expert
+// they are bound by the tensor cores, with a few rows by reading the weights.
+//
+// * A pair of CTAs (a cluster of 2 on one TPC) works on one tile with tcgen05.mma.cta_group::2.
+//   The 256 rows of the tile's M are weight rows ("features": 128 per CTA), and its N, 32 to 256 in
+//   steps of 32, are rows of one expert.  So the ragged dimension is the one that the instruction
+//   takes in small steps: a group of 20 rows costs an N of 32, not a tile of 128 or 256, and the
+//   same kernel serves single tokens.  Each CTA loads its 128 features and half of the N rows:
+//   32 KB per 64-deep step at N = 256, which the L2 can deliver (64 B/clk per SM) while the
+//   pair's tensor cores take 512 clocks for it.
+// * The weight gradients sum over an expert's rows instead: M and N are the two weight dimensions.
+//   Rows that follow the group in the last 64-deep step must not count, whatever they hold: a
+//   warp overwrites them with zeros in shared memory, up to the 16 that one instruction takes.
+// * Warp 0 issues the TMA loads into a ring of stages, warp 1 of the leading CTA the matrix
+//   instructions, warp 2 clears tails, warps 4 to 7 move finished accumulators out of TMEM, where
+//   two tiles' accumulators fit, so that they overlap the next tile's products.
+// * Every pair walks the tile list by itself (tile t, t + pairs, ...): the row counts are read on
+//   the device, and no CTA waits for another outside its pair.
+//
+// Roundings to the 16-bit type: h, dg and du, once each, because they are operands of the next
+// product.  The projections g and u that the backward pass reads are kept in fp32: in 16 bits they
+// made dx and dw_in 1.8 times as far off as one rounding of the result does, against 1.4 times now.
+//
+// Every wait is bounded: one that runs out sets *status and ends the kernel.
 #include "collective/operators.hpp"
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 namespace ugdr::coll {
 namespace {
 
-constexpr int kTile = 64, kDepth = 16, kBlock = 256;
+constexpr int kThreads = 256;       // 8 warps
+constexpr int kHalf = 128;          // features of a tile per CTA: the lanes of TMEM
+constexpr int kPairFeatures = 256;
+constexpr int kMaxN = 256;
+constexpr int kStepN = 32;
+constexpr int kDepth = 64;          // elements per stage along the summed dimension: 128 bytes
+constexpr int kSmallBox = 16;       // rows of the small TMA box: half of kStepN
+constexpr int kStages = 5;
+constexpr int kBand = 8;            // row tiles that run through all features before the next
+constexpr uint32_t kOperandBytes = kHalf * kDepth * 2;  // one CTA's half of A, or of B, in a stage
+constexpr int kStagingRow = kHalf + 4;                  // floats; the 4 keep 16-byte reads apart
+constexpr uint32_t kStagingBytes = 32 * kStagingRow * 4;
+constexpr uint64_t kWaitNs = 5ull * 1000 * 1000 * 1000;
 
-__device__ __forceinline__ float load(const __half *p) { return __half2float(*p); }
-__device__ __forceinline__ float load(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void store(__half *p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void store(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
+enum Product { kUp, kDown, kBack, kInput, kGradOut, kGradIn };
+template <Product P> constexpr bool kWeightGrad = P == kGradOut || P == kGradIn;
+// Whether A's features lie next to each other in memory (else its summed dimension does).
+template <Product P> constexpr bool kFeaturesInner = P != kUp && P != kDown;
+
+struct Shape {
+    const int32_t *counts;
+    unsigned int *status;
+    int rows, nexp, hidden, inner, act;
+};
+
+struct Shared {
+    alignas(8) uint64_t full[kStages], empty[kStages], tail[kStages], tmem_full[2], tmem_empty[2];
+    uint32_t tmem;
+    int aborted;
+    long long scan[kThreads / 32];
+};
+constexpr size_t shared_bytes(int nexp) {
+    return 1024 + kStages * 2 * kOperandBytes + 2 * kStagingBytes + sizeof(Shared) + (size_t(nexp) + 1) * 4;
+}
+static_assert(shared_bytes(UGDR_X_EXPERTS_MAX) <= 232448, "227 KB of shared memory per CTA");
+
+// ---- PTX ---------------------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return uint32_t(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ uint64_t gtime() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+__device__ __forceinline__ uint32_t cta_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// The same shared address in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_cluster(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n.reg .pred p;\n"
+                 "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+                 "selp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(done)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    return done != 0;
+}
+// Waits until the barrier's phase of `parity` is over.  False: the wait, or another of this CTA,
+// ran out, and the caller gives up.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, Shared &sh, unsigned int *status) {
+    uint64_t since = 0;
+    for (uint32_t spins = 1; !mbar_try(bar, parity); ++spins) {
+        if (spins % 64 != 0) continue;
+        if (*reinterpret_cast<volatile int *>(&sh.aborted)) return false;
+        const uint64_t now = gtime();
+        if (since == 0) since = now;
+        if (now - since > kWaitNs) {
+            *reinterpret_cast<volatile int *>(&sh.aborted) = 1;
+            atomicExch(status, 1u);
+            return false;
+        }
+    }
+    return true;
+}
+
+// TMA loads into this CTA; the bytes are counted by `bar`, here or in the pair's other CTA.
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+                 "[%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+                 "l"(map), "r"(bar), "r"(c0), "r"(c1)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2) {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+                 "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+                 "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2,
+                                         int c3) {
+    asm volatile("cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+                 "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+                 "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+                 : "memory");
+}
+
+// Operand descriptor for 128-byte swizzled tiles (rows of 128 bytes, atoms of 8 rows).  With the
+// summed dimension inner, 8 features to an atom and 1024 bytes to the next 8.  With the features
+// inner, 64 of them to an atom of 8 summed positions, 1024 bytes to the next 8 positions and one
+// tile of 64 x 128 bytes to the next 64 features.
+template <bool FEATURES_INNER> __device__ __forceinline__ uint64_t operand(uint32_t addr) {
+    const uint64_t leading = FEATURES_INNER ? kDepth * 128 / 16 : 1, stride = 1024 / 16;
+    return uint64_t(addr >> 4) | leading << 16 | stride << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+// From one instruction's 16 summed positions to the next's, in the descriptor's address field.
+template <bool FEATURES_INNER> constexpr uint64_t kOperandStep = FEATURES_INNER ? 16 * 128 / 16 : 16 * 2 / 16;
+
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+                 : "memory");
+}
+// Arrives on `bar` of both CTAs once the instructions issued before are done.
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                     bar),
+                 "h"(uint16_t(3))
+                 : "memory");
+}
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+// 32 columns of this warp's 32 TMEM lanes: v[j] is column j of lane threadIdx.x % 32.
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
+    uint32_t *r = reinterpret_cast<uint32_t *>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+                   "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+                   "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+                   "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// Whether all four epilogue warps say so: one that gives up takes the others along.
+__device__ __forceinline__ bool epilogue_all(bool ok) {
+    uint32_t all;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\n"
+                 "bar.red.and.pred q, 1, 128, p;\nselp.u32 %0, 1, 0, q;\n}"
+                 : "=r"(all)
+                 : "r"(uint32_t(ok))
+                 : "memory");
+    return all != 0;
+}
+
+// ---- tiles -------------------------------------------------------------------------------------
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+struct Tile {
+    int expert;
+    int feature;  // first of the pair's features
+    int part;     // kGradIn: 0 the gate's, 1 the up projection's weights
+    int first;    // rows products: the tile's first row.  Weight gradients: the group's
+    int rows;     // likewise, of the tile or the group
+    int column;   // weight gradients: first of the N
+};
+
+// Features of a tile of the pair: with kUp 128 of the gate and the same 128 of the up projection.
+template <Product P> constexpr int kTileFeatures = P == kUp ? kPairFeatures / 2 : kPairFeatures;
+
+// Walks the tile list in order: next() finds tile t for increasing t.
+template <Product P> struct Tiles {
+    const int *first;  // first row of each expert's group, and the end of the last
+    int nexp, mtiles, mparts, ntiles;
+    int expert, base, size;
+
+    __device__ Tiles(const Shape &m, const int *first_) : first(first_), nexp(m.nexp), expert(-1), base(0), size(0) {
+        const int features = P == kUp || P == kBack || P == kGradIn ? m.inner : m.hidden;
+        mparts = ceil_div(features, kTileFeatures<P>);
+        mtiles = P == kGradIn ? 2 * mparts : mparts;
+        ntiles = P == kGradOut ? ceil_div(m.inner, kMaxN) : P == kGradIn ? ceil_div(m.hidden, kMaxN) : 0;
+    }
+    __device__ __forceinline__ bool next(int t, Tile &out) {
+        int n = 0;
+        while (t >= base + size) {
+            if (++expert >= nexp) return false;
+            base += size;
+            n = first[expert + 1] - first[expert];
+            size = mtiles * (kWeightGrad<P> ? ntiles : ceil_div(n, kMaxN));
+        }
+        n = first[expert + 1] - first[expert];
+        // Bands of kBand N tiles; inside, all N tiles of one feature tile before the next, so that
+        // pairs that run together share weights and rows in the L2.
+        const int columns = kWeightGrad<P> ? ntiles : ceil_div(n, kMaxN);
+        const int local = t - base, band = local / (kBand * mtiles), in_band = local - band * kBand * mtiles;
+        const int width = min(kBand, columns - band * kBand);
+        const int mtile = in_band / width, ntile = band * kBand + in_band - mtile * width;
+        out.expert = expert;
+        out.part = P == kGradIn ? mtile / mparts : 0;
+        out.feature = (mtile - out.part * mparts) * kTileFeatures<P>;
+        if (kWeightGrad<P>) {
+            out.first = first[expert];
+            out.rows = n;
+            out.column = ntile * kMaxN;
+        } else {
+            // Tiles of about the same size, none above kMaxN, all but the last a multiple of kStepN.
+            const int per = ceil_div(ceil_div(n, columns), kStepN) * kStepN;
+            out.first = first[expert] + ntile * per;
+            out.rows = min(per, n - ntile * per);
+            out.column = 0;
+        }
+        return true;
+    }
+};
+
+template <Product P> __device__ __forceinline__ int steps_of(const Shape &m, const Tile &t) {
+    if (kWeightGrad<P>) return ceil_div(t.rows, kDepth);
+    if (P == kInput) return 2 * ceil_div(m.inner, kDepth);
+    return ceil_div(P == kDown ? m.inner : m.hidden, kDepth);
+}
+
+// First rows of the groups into first[0 .. nexp]: a scan over the block's threads.
+__device__ void scan_counts(const Shape &m, Shared &sh, int *first) {
+    const int per = ceil_div(m.nexp, kThreads), lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int e0 = min(m.nexp, int(threadIdx.x) * per), e1 = min(m.nexp, e0 + per);
+    long long own = 0;
+    bool bad = false;
+    for (int e = e0; e < e1; ++e) {
+        const int c = m.counts[e];
+        bad |= c < 0;
+        own += max(c, 0);
+    }
+    long long upto = own;
+    for (int o = 1; o < 32; o *= 2) {
+        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) sh.scan[warp] = upto;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) upto += sh.scan[w];
+    long long at = upto - own;
+    for (int e = e0; e < e1; ++e) {
+        first[e] = int(min(at, (long long)m.rows));
+        at += max(m.counts[e], 0);
+    }
+    if (threadIdx.x == kThreads - 1) {
+        first[m.nexp] = int(min(upto, (long long)m.rows));
+        bad |= upto > m.rows;
+    }
+    if (bad && blockIdx.x == 0) atomicExch(m.status, 2u);
+}
+
+// ---- elements ----------------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <typename T> __device__ __forceinline__ void store8(T *p, const float *v) {
+    *reinterpret_cast<uint4 *>(p) =
+        make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
+}
+__device__ __forceinline__ void store8(float *p, const float *v) {
+    reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void load8(const float *p, float *v) {
+    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
 
 // The activation and its derivative.
 __device__ __forceinline__ float act(float g, int kind) {
@@ -34,190 +345,384 @@ __device__ __forceinline__ float act_grad(float g, int kind) {
     return 0.5f * (1.f + erff(g * 0.70710678f)) + g * 0.39894228f * expf(-0.5f * g * g);
 }
 
-struct Shape {
-    const int32_t *counts;
-    unsigned int *status;
-    int64_t rows;
-    int nexp, hidden, inner, act;
+// ---- the kernel --------------------------------------------------------------------------------
+
+struct Maps {
+    CUtensorMap a, b, b_small;
 };
 
-struct Rows {
-    int expert;
-    int64_t first, end;  // rows [first, end), of one expert
-};
-
-// Row range of expert e.
-__device__ Rows rows_of(const Shape &m, int e) {
-    int64_t at = 0;
-    for (int i = 0; i < e; ++i) at += max(m.counts[i], 0);
-    at = min(at, m.rows);
-    return {e, at, min(at + max(m.counts[e], 0), m.rows)};
-}
-
-// The `tile`-th piece of at most kTile rows of one expert (expert -1: there are fewer).
-__device__ Rows row_tile(const Shape &m, int tile) {
-    int64_t at = 0;
-    bool bad = false;
-    Rows r{-1, 0, 0};
-    for (int e = 0; e < m.nexp; ++e) {
-        const int64_t n = m.counts[e];
-        bad |= n < 0;
-        const int64_t end = min(at + max(n, int64_t(0)), m.rows);
-        bad |= at + n > m.rows;
-        const int tiles = int((end - at + kTile - 1) / kTile);
-        if (r.expert < 0 && tile < tiles) {
-            r = {e, at + int64_t(tile) * kTile, 0};
-            r.end = min(r.first + kTile, end);
-        }
-        tile -= tiles;
-        at = end;
-    }
-    if (bad) atomicExch(m.status, 2u);
-    return r;
-}
-
-enum Product { kUp, kDown, kBack, kInput };
-
-// One tile of a product whose rows are the experts' rows.
-//   kUp     out = h = a(x Wg^T) * (x Wu^T)  (and gu)     a_rows = x
-//   kDown   out = y = h Wo^T                             a_rows = h
-//   kBack   out = dgu from dh = dy Wo and gu             a_rows = dy
-//   kInput  out = dx = dgu (Wg; Wu)                      a_rows = dgu
 template <typename T, Product P>
-__global__ void __launch_bounds__(kBlock) rows_kernel(Shape m, const T *a_rows, const T *w, T *out, T *gu) {
-    constexpr int kB = P == kUp ? 2 : 1;
-    __shared__ float sa[kDepth][kTile + 1], sb[kB][kDepth][kTile + 1];
-    __shared__ Rows tile;
-    if (threadIdx.x == 0) tile = row_tile(m, blockIdx.y);
-    __syncthreads();
-    const Rows r = tile;
-    if (r.expert < 0) return;
-    const int H = m.hidden, F = m.inner;
-    const int features = P == kUp || P == kBack ? F : H;
-    const int depth = P == kUp || P == kBack ? H : P == kDown ? F : 2 * F;
-    const T *we = w + int64_t(r.expert) * H * F * (P == kUp || P == kInput ? 2 : 1);
-    const int f0 = blockIdx.x * kTile, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    float acc[kB][4][4] = {};
-    for (int k0 = 0; k0 < depth; k0 += kDepth) {
-        for (int i = threadIdx.x; i < kTile * kDepth; i += kBlock) {
-            const int k = k0 + i % kDepth, row = i / kDepth;
-            sa[i % kDepth][row] =
-                k < depth && r.first + row < r.end ? load(a_rows + (r.first + row) * int64_t(depth) + k) : 0.f;
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    expert_kernel(const __grid_constant__ Maps maps, const Shape m, T *out, float *gu) {
+    extern __shared__ uint8_t raw[];
+    uint8_t *tiles_mem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);
+    float *staging = reinterpret_cast<float *>(tiles_mem + kStages * 2 * kOperandBytes);
+    Shared &sh = *reinterpret_cast<Shared *>(reinterpret_cast<uint8_t *>(staging) + 2 * kStagingBytes);
+    int *first = reinterpret_cast<int *>(&sh + 1);
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = cta_rank();
+    const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+    const uint32_t stage0 = smem_addr(tiles_mem);
+    constexpr bool kInnerA = kFeaturesInner<P>, kInnerB = kWeightGrad<P>;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(smem_addr(&sh.full[s]), 2);   // both CTAs' loads, counted in the leading CTA
+            mbar_init(smem_addr(&sh.empty[s]), 1);
+            mbar_init(smem_addr(&sh.tail[s]), 1);
         }
-        for (int b = 0; b < kB; ++b) {
-            for (int i = threadIdx.x; i < kTile * kDepth; i += kBlock) {
-                // Weights with the depth innermost (kUp, kDown), or the feature.
-                const bool inner_depth = P == kUp || P == kDown;
-                const int kk = inner_depth ? i % kDepth : i / kTile, ff = inner_depth ? i / kDepth : i % kTile;
-                const int k = k0 + kk, f = f0 + ff;
-                float v = 0.f;
-                if (k < depth && f < features)
-                    v = load(we + (inner_depth ? (int64_t(b) * features + f) * depth + k : int64_t(k) * features + f));
-                sb[b][kk][ff] = v;
-            }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(smem_addr(&sh.tmem_full[s]), 1);
+            mbar_init(smem_addr(&sh.tmem_empty[s]), 8);  // 4 epilogue warps of each CTA
         }
-        __syncthreads();
-        for (int k = 0; k < kDepth; ++k)
-            for (int b = 0; b < kB; ++b)
-                for (int i = 0; i < 4; ++i)
-                    for (int j = 0; j < 4; ++j) acc[b][i][j] += sa[k][ty * 4 + i] * sb[b][k][tx + 16 * j];
-        __syncthreads();
+        sh.aborted = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    for (int i = 0; i < 4; ++i) {
-        const int64_t row = r.first + ty * 4 + i;
-        if (row >= r.end) continue;
-        for (int j = 0; j < 4; ++j) {
-            const int f = f0 + tx + 16 * j;
-            if (f >= features) continue;
-            if constexpr (P == kUp) {
-                if (gu != nullptr) {
-                    store(gu + row * 2 * F + f, acc[0][i][j]);
-                    store(gu + row * 2 * F + F + f, acc[kB - 1][i][j]);
+    scan_counts(m, sh, first);
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sh.tmem))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    cluster_sync();
+    fence_after();
+    const uint32_t tmem = sh.tmem;
+
+    if (warp == 0 && lane == 0) {
+        // Loads: this CTA's features and its half of the rows (or columns), stage after stage.
+        Tiles<P> tiles(m, first);
+        Tile t;
+        uint32_t it = 0;
+        bool go = true;
+        for (int at = pair; go && tiles.next(at, t); at += pairs) {
+            const int steps = steps_of<P>(m, t), n = ceil_div(t.rows, kStepN) * kStepN;
+            const int half = kWeightGrad<P> ? kHalf : n / 2;
+            const uint32_t bytes = kOperandBytes + uint32_t(half) * kDepth * 2;
+            const int feature = t.feature + int(rank) * (kTileFeatures<P> / 2);
+            for (int k = 0; k < steps; ++k, ++it) {
+                const uint32_t s = it % kStages;
+                if (!mbar_wait(smem_addr(&sh.empty[s]), (it / kStages + 1) & 1, sh, m.status)) {
+                    go = false;
+                    break;
                 }
-                store(out + row * F + f, act(acc[0][i][j], m.act) * acc[kB - 1][i][j]);
-            } else if constexpr (P == kBack) {
-                const float g = load(gu + row * 2 * F + f), u = load(gu + row * 2 * F + F + f);
-                store(out + row * 2 * F + f, acc[0][i][j] * u * act_grad(g, m.act));
-                store(out + row * 2 * F + F + f, acc[0][i][j] * act(g, m.act));
+                const uint32_t a = stage0 + s * 2 * kOperandBytes, b = a + kOperandBytes;
+                // A last step that reaches past the group goes to the warp that clears its tail.
+                const bool tail = kWeightGrad<P> && (k + 1) * kDepth > t.rows;
+                uint32_t bar = map_to(smem_addr(&sh.full[s]), 0);
+                if (tail) bar = map_to(smem_addr(&sh.tail[s]), rank);
+                mbar_expect_cluster(bar, bytes);
+                const int depth = k * kDepth;
+                if constexpr (P == kUp) {
+                    tma_load(a, &maps.a, bar, depth, feature, 0, t.expert);
+                } else if constexpr (P == kDown) {
+                    tma_load(a, &maps.a, bar, depth, feature, t.expert);
+                } else {
+                    for (int c = 0; c < 2; ++c) {
+                        const uint32_t dst = a + uint32_t(c) * kOperandBytes / 2;
+                        const int f = feature + c * 64;
+                        if constexpr (P == kBack) {
+                            tma_load(dst, &maps.a, bar, f, depth, t.expert);
+                        } else if constexpr (P == kInput) {
+                            const int part = k >= steps / 2;
+                            tma_load(dst, &maps.a, bar, f, depth - part * (steps / 2) * kDepth, part, t.expert);
+                        } else if constexpr (P == kGradOut) {
+                            tma_load(dst, &maps.a, bar, f, t.first + depth);
+                        } else {
+                            tma_load(dst, &maps.a, bar, f, t.part, t.first + depth);
+                        }
+                    }
+                }
+                if constexpr (kWeightGrad<P>) {
+                    for (int c = 0; c < 2; ++c)
+                        tma_load(b + uint32_t(c) * kOperandBytes / 2, &maps.b, bar,
+                                 t.column + int(rank) * kHalf + c * 64, t.first + depth);
+                } else {
+                    const bool whole = half == kHalf;
+                    const int box = whole ? kHalf : kSmallBox, row = t.first + int(rank) * half;
+                    const CUtensorMap *map = whole ? &maps.b : &maps.b_small;
+                    for (int r = 0; r < half; r += box) {
+                        const uint32_t dst = b + uint32_t(r) * kDepth * 2;
+                        if constexpr (P == kInput) {
+                            const int part = k >= steps / 2;
+                            tma_load(dst, map, bar, depth - part * (steps / 2) * kDepth, part, row + r);
+                        } else {
+                            tma_load(dst, map, bar, depth, row + r);
+                        }
+                    }
+                }
+            }
+        }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        // Matrix instructions of the pair.
+        constexpr uint32_t kType = std::is_same_v<T, __nv_bfloat16> ? 1 : 0;
+        constexpr uint32_t kBase = 1u << 4 | kType << 7 | kType << 10 | uint32_t(kInnerA) << 15 |
+                                   uint32_t(kInnerB) << 16 | uint32_t(kPairFeatures / 16) << 24;
+        Tiles<P> tiles(m, first);
+        Tile t;
+        uint32_t it = 0, acc = 0;
+        bool go = true;
+        for (int at = pair; go && tiles.next(at, t); at += pairs) {
+            const int steps = steps_of<P>(m, t);
+            if (steps == 0) continue;
+            const int n = kWeightGrad<P> ? kMaxN : ceil_div(t.rows, kStepN) * kStepN;
+            const uint32_t idesc = kBase | uint32_t(n / 8) << 17;
+            const uint32_t d = tmem + (acc & 1) * kMaxN;
+            if (!mbar_wait(smem_addr(&sh.tmem_empty[acc & 1]), (acc / 2 + 1) & 1, sh, m.status)) break;
+            fence_after();
+            for (int k = 0; k < steps; ++k, ++it) {
+                const uint32_t s = it % kStages;
+                if (!mbar_wait(smem_addr(&sh.full[s]), (it / kStages) & 1, sh, m.status)) {
+                    go = false;
+                    break;
+                }
+                fence_after();
+                const uint32_t addr = stage0 + s * 2 * kOperandBytes;
+                const uint64_t a = operand<kInnerA>(addr), b = operand<kInnerB>(addr + kOperandBytes);
+                int parts = kDepth / 16;
+                if (kWeightGrad<P>) parts = min(parts, ceil_div(t.rows - k * kDepth, 16));
+                for (int i = 0; i < parts; ++i)
+                    mma(d, a + i * kOperandStep<kInnerA>, b + i * kOperandStep<kInnerB>, idesc, k + i > 0);
+                mma_commit(smem_addr(&sh.empty[s]));
+            }
+            if (go) mma_commit(smem_addr(&sh.tmem_full[acc & 1]));
+            ++acc;
+        }
+    } else if (warp == 2 && kWeightGrad<P>) {
+        // Tails: the rows behind the group in its last step, up to the next 16, become zeros.
+        Tiles<P> tiles(m, first);
+        Tile t;
+        uint32_t it = 0, phases = 0;
+        for (int at = pair; tiles.next(at, t); at += pairs) {
+            const int steps = steps_of<P>(m, t), last = t.rows % kDepth;
+            it += uint32_t(steps);
+            if (last == 0) continue;
+            const uint32_t s = (it - 1) % kStages;
+            if (!mbar_wait(smem_addr(&sh.tail[s]), phases >> s & 1, sh, m.status)) break;
+            phases ^= 1u << s;
+            uint8_t *stage = tiles_mem + s * 2 * kOperandBytes;
+            const int clear = ceil_div(last, 16) * 16 - last;  // rows of 128 bytes, in each of 4 tiles
+            for (int i = lane; i < clear * 4 * 8; i += 32) {
+                const int tile = i / (clear * 8), piece = i % (clear * 8);
+                reinterpret_cast<uint4 *>(stage + tile * (kDepth * 128) + last * 128)[piece] = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(map_to(smem_addr(&sh.full[s]), 0));
+            __syncwarp();
+        }
+    } else if (warp >= 4) {
+        // Finished accumulators.  This warp's TMEM lanes are features 32 (warp % 4) ... + 31.
+        const int quarter = warp % 4;
+        const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
+        Tiles<P> tiles(m, first);
+        Tile t;
+        uint32_t acc = 0, chunk = 0;
+        for (int at = pair; tiles.next(at, t); at += pairs) {
+            const bool none = steps_of<P>(m, t) == 0;
+            if (!none) {
+                if (!epilogue_all(mbar_wait(smem_addr(&sh.tmem_full[acc & 1]), (acc / 2) & 1, sh, m.status))) break;
+                fence_after();
+            }
+            const uint32_t columns = lanes + (acc & 1) * kMaxN;
+            const int feature = t.feature + int(rank) * (kTileFeatures<P> / 2);
+            if constexpr (kWeightGrad<P>) {
+                // A thread has one row of the gradient and writes its columns.
+                const int width = P == kGradOut ? m.inner : m.hidden, height = P == kGradOut ? m.hidden : m.inner;
+                const int f = feature + quarter * 32 + lane;
+                T *row = out + ((int64_t(t.expert) * (P == kGradIn ? 2 : 1) + t.part) * height + f) * width + t.column;
+                for (int c = 0; c < kMaxN; c += 32) {
+                    float v[32];
+                    if (none) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = 0.f;
+                    } else {
+                        tmem_load(columns + c, v);
+                    }
+                    if (f < height) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 8)
+                            if (t.column + c + j < width) store8(row + c + j, v + j);
+                    }
+                }
             } else {
-                store(out + row * features + f, acc[0][i][j]);
+                // 32 rows at a time, turned around in shared memory: then 4 lanes hold a row's
+                // features, 8 next to each other per lane.
+                for (int c = 0; c < t.rows; c += 32, ++chunk) {
+                    float v[32];
+                    tmem_load(columns + c, v);
+                    float *buffer = staging + (chunk & 1) * (kStagingBytes / 4);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) buffer[j * kStagingRow + quarter * 32 + lane] = v[j];
+                    epilogue_sync();
+                    const int r = quarter * 8 + lane / 4;
+                    const float *from = buffer + r * kStagingRow;
+                    if (c + r < t.rows) {
+                        const int64_t row = t.first + c + r;
+                        constexpr int kFeatures = P == kUp ? 64 : 128;
+#pragma unroll
+                        for (int i = lane % 4 * 8; i < kFeatures; i += 32) {
+                            const int f = feature + i;
+                            float a[8], b[8], w[8];
+                            load8(from + i, a);
+                            if constexpr (P == kUp) {
+                                if (f >= m.inner) break;
+                                load8(from + 64 + i, b);
+                                if (gu != nullptr) {
+                                    store8(gu + row * 2 * m.inner + f, a);
+                                    store8(gu + row * 2 * m.inner + m.inner + f, b);
+                                }
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) w[j] = act(a[j], m.act) * b[j];
+                                store8(out + row * m.inner + f, w);
+                            } else if constexpr (P == kBack) {
+                                if (f >= m.inner) break;
+                                float g[8], u[8];
+                                load8(gu + row * 2 * m.inner + f, g);
+                                load8(gu + row * 2 * m.inner + m.inner + f, u);
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    w[j] = a[j] * u[j] * act_grad(g[j], m.act);
+                                    b[j] = a[j] * act(g[j], m.act);
+                                }
+                                store8(out + row * 2 * m.inner + f, w);
+                                store8(out + row * 2 * m.inner + m.inner + f, b);
+                            } else {
+                                if (f >= m.hidden) break;
+                                store8(out + row * m.hidden + f, a);
+                            }
+                        }
+                    }
+                }
+            }
+            if (!none) {
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(map_to(smem_addr(&sh.tmem_empty[acc & 1]), 0));
+                ++acc;
             }
         }
     }
-}
-
-// One tile of an expert's weight gradient: out[m][n] = sum over its rows of a[row][m] * b[row][n].
-template <typename T>
-__global__ void __launch_bounds__(kBlock) weights_kernel(Shape m, const T *a, int am, const T *b, int bn, T *out) {
-    __shared__ float sa[kDepth][kTile], sb[kDepth][kTile];
-    __shared__ Rows range;
-    if (threadIdx.x == 0) range = rows_of(m, blockIdx.z);
     __syncthreads();
-    const Rows r = range;
-    const int m0 = blockIdx.y * kTile, n0 = blockIdx.x * kTile, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    float acc[4][4] = {};
-    for (int64_t r0 = r.first; r0 < r.end; r0 += kDepth) {
-        for (int i = threadIdx.x; i < kTile * kDepth; i += kBlock) {
-            const int64_t row = r0 + i / kTile;
-            const int c = i % kTile;
-            sa[i / kTile][c] = row < r.end && m0 + c < am ? load(a + row * am + m0 + c) : 0.f;
-            sb[i / kTile][c] = row < r.end && n0 + c < bn ? load(b + row * bn + n0 + c) : 0.f;
-        }
-        __syncthreads();
-        for (int k = 0; k < kDepth; ++k)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) acc[i][j] += sa[k][ty * 4 + i] * sb[k][tx + 16 * j];
-        __syncthreads();
+    if (sh.aborted) {  // loads and instructions that are still under way end within this time
+        for (const uint64_t since = gtime(); gtime() - since < 2'000'000;) __nanosleep(1000);
     }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int mm = m0 + ty * 4 + i, nn = n0 + tx + 16 * j;
-            if (mm < am && nn < bn) store(out + (int64_t(r.expert) * am + mm) * bn + nn, acc[i][j]);
-        }
+    fence_before();
+    cluster_sync();
+    if (warp == 2) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
 }
 
-Shape shape_of(const ugdr_x_experts &m) {
-    return {m.counts, m.status, int64_t(m.rows), m.nexp, m.hidden, m.inner, m.act};
+// ---- launches ----------------------------------------------------------------------------------
+
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                              const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+    static const EncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return EncodeFn(nullptr);
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
 }
 
-unsigned tiles(int64_t n) { return unsigned((n + kTile - 1) / kTile); }
+// A dense tensor of 16-bit elements, the innermost dimension first; boxes of 64 elements (128
+// swizzled bytes) by `box` in the other dimensions.  Reads past an end of a dimension give zeros.
+struct Dense {
+    const void *base;
+    int rank;
+    cuuint64_t dims[4];
+    cuuint32_t box[4];
+};
+
+template <typename T> bool encode(CUtensorMap *map, const Dense &d) {
+    cuuint64_t strides[3];
+    cuuint32_t ones[4] = {1, 1, 1, 1};
+    cuuint64_t bytes = 2;
+    for (int i = 0; i + 1 < d.rank; ++i) strides[i] = bytes *= d.dims[i];
+    const auto type = std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return encode_fn() != nullptr &&
+           encode_fn()(map, type, cuuint32_t(d.rank), const_cast<void *>(d.base), d.dims, strides, d.box, ones,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// One product.  `a` and `b` are its operands: the weights and the rows, or the two row tensors of a
+// weight gradient.
+template <typename T, Product P>
+cudaError_t launch(const ugdr_x_experts &m, const void *a, const void *b, void *out, float *gu, cudaStream_t s) {
+    const cuuint64_t H = cuuint64_t(m.hidden), F = cuuint64_t(m.inner), R = m.rows, E = cuuint64_t(m.nexp);
+    Dense da, db;
+    if (P == kUp)
+        da = {a, 4, {H, F, 2, E}, {64, 64, 2, 1}};
+    else if (P == kInput)
+        da = {a, 4, {H, F, 2, E}, {64, 64, 1, 1}};
+    else if (P == kDown)
+        da = {a, 3, {F, H, E}, {64, 128, 1}};
+    else if (P == kBack)
+        da = {a, 3, {F, H, E}, {64, 64, 1}};
+    else if (P == kGradOut)
+        da = {a, 2, {H, R}, {64, 64}};
+    else
+        da = {a, 3, {F, 2, R}, {64, 1, 64}};
+    const cuuint32_t rows = kWeightGrad<P> ? 64 : kHalf;
+    if (P == kInput)
+        db = {b, 3, {F, 2, R}, {64, 1, rows}};
+    else
+        db = {b, 2, {P == kUp || P == kBack || P == kGradIn ? H : F, R}, {64, rows}};
+    Maps maps;
+    if (!encode<T>(&maps.a, da) || !encode<T>(&maps.b, db)) return cudaErrorInvalidValue;
+    db.box[db.rank - 1] = kSmallBox;
+    if (!encode<T>(&maps.b_small, db)) return cudaErrorInvalidValue;
+
+    int device = 0, sms = 0;
+    if (cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return e;
+    if (cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device); e != cudaSuccess) return e;
+    const size_t bytes = shared_bytes(m.nexp);
+    auto *kernel = expert_kernel<T, P>;
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             int(shared_bytes(UGDR_X_EXPERTS_MAX)));
+        e != cudaSuccess)
+        return e;
+    const Shape shape{m.counts, m.status, int(m.rows), m.nexp, m.hidden, m.inner, m.act};
+    kernel<<<sms / 2 * 2, kThreads, bytes, s>>>(maps, shape, static_cast<T *>(out), gu);
+    return cudaGetLastError();
+}
 
 template <typename T>
-int forward(const ugdr_x_experts &m, const void *x, void *y, void *h, void *gu, cudaStream_t s) {
-    const Shape sh = shape_of(m);
-    const unsigned row_tiles = tiles(int64_t(m.rows)) + unsigned(m.nexp);
-    rows_kernel<T, kUp><<<dim3(tiles(m.inner), row_tiles), kBlock, 0, s>>>(
-        sh, static_cast<const T *>(x), static_cast<const T *>(m.w_in), static_cast<T *>(h), static_cast<T *>(gu));
-    rows_kernel<T, kDown><<<dim3(tiles(m.hidden), row_tiles), kBlock, 0, s>>>(
-        sh, static_cast<const T *>(h), static_cast<const T *>(m.w_out), static_cast<T *>(y), nullptr);
-    return int(cudaGetLastError());
+int forward(const ugdr_x_experts &m, const void *x, void *y, void *h, float *gu, cudaStream_t s) {
+    cudaError_t e = launch<T, kUp>(m, m.w_in, x, h, gu, s);
+    if (e == cudaSuccess) e = launch<T, kDown>(m, m.w_out, h, y, nullptr, s);
+    return int(e);
 }
 
 template <typename T>
-int backward(const ugdr_x_experts &m, const void *dy, const void *x, const void *h, const void *gu, void *dgu,
+int backward(const ugdr_x_experts &m, const void *dy, const void *x, const void *h, const float *gu, void *dgu,
              void *dx, void *dw_in, void *dw_out, cudaStream_t s) {
-    const Shape sh = shape_of(m);
-    const unsigned row_tiles = tiles(int64_t(m.rows)) + unsigned(m.nexp), e = unsigned(m.nexp);
-    rows_kernel<T, kBack><<<dim3(tiles(m.inner), row_tiles), kBlock, 0, s>>>(
-        sh, static_cast<const T *>(dy), static_cast<const T *>(m.w_out), static_cast<T *>(dgu),
-        const_cast<T *>(static_cast<const T *>(gu)));
-    weights_kernel<T><<<dim3(tiles(m.inner), tiles(m.hidden), e), kBlock, 0, s>>>(
-        sh, static_cast<const T *>(dy), m.hidden, static_cast<const T *>(h), m.inner, static_cast<T *>(dw_out));
-    weights_kernel<T><<<dim3(tiles(m.hidden), tiles(2 * int64_t(m.inner)), e), kBlock, 0, s>>>(
-        sh, static_cast<const T *>(dgu), 2 * m.inner, static_cast<const T *>(x), m.hidden, static_cast<T *>(dw_in));
+    cudaError_t e = launch<T, kBack>(m, m.w_out, dy, dgu, const_cast<float *>(gu), s);
+    if (e == cudaSuccess) e = launch<T, kGradOut>(m, dy, h, dw_out, nullptr, s);
+    if (e == cudaSuccess) e = launch<T, kGradIn>(m, dgu, x, dw_in, nullptr, s);
     // Last, so that dx may be dy or x itself.
-    rows_kernel<T, kInput><<<dim3(tiles(m.hidden), row_tiles), kBlock, 0, s>>>(
-        sh, static_cast<const T *>(dgu), static_cast<const T *>(m.w_in), static_cast<T *>(dx), nullptr);
-    return int(cudaGetLastError());
+    if (e == cudaSuccess) e = launch<T, kInput>(m, m.w_in, dgu, dx, nullptr, s);
+    return int(e);
 }
 
 }  // namespace
 
-int launch_expert_ffn(const ugdr_x_experts &m, const void *x, void *y, void *h, void *gu, cudaStream_t s) {
+int launch_expert_ffn(const ugdr_x_experts &m, const void *x, void *y, void *h, float *gu, cudaStream_t s) {
     return m.type == UGDR_X_TYPE_BF16 ? forward<__nv_bfloat16>(m, x, y, h, gu, s) : forward<__half>(m, x, y, h, gu, s);
 }
 
-int launch_expert_ffn_backward(const ugdr_x_experts &m, const void *dy, const void *x, const void *h, const void *gu,
+int launch_expert_ffn_backward(const ugdr_x_experts &m, const void *dy, const void *x, const void *h, const float *gu,
                                void *dgu, void *dx, void *dw_in, void *dw_out, cudaStream_t s) {
     return m.type == UGDR_X_TYPE_BF16 ? backward<__nv_bfloat16>(m, dy, x, h, gu, dgu, dx, dw_in, dw_out, s)
                                       : backward<__half>(m, dy, x, h, gu, dgu, dx, dw_in, dw_out, s);

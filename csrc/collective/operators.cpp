@@ -21,7 +21,7 @@ size_t element_bytes(int type) { return type == UGDR_X_TYPE_FP32 ? 4 : 2; }
 
 extern "C" {
 
-int ugdr_x_expert_ffn(const ugdr_x_experts *m, const void *x, void *y, void *h, void *gu, void *stream) {
+int ugdr_x_expert_ffn(const ugdr_x_experts *m, const void *x, void *y, void *h, float *gu, void *stream) {
     if (!valid(m)) return int(cudaErrorInvalidValue);
     if (m->rows == 0) return int(cudaSuccess);
     if (!aligned16(x) || !aligned16(y) || !aligned16(h) || (gu != nullptr && !aligned16(gu)))
@@ -29,7 +29,7 @@ int ugdr_x_expert_ffn(const ugdr_x_experts *m, const void *x, void *y, void *h, 
     return ugdr::coll::launch_expert_ffn(*m, x, y, h, gu, static_cast<cudaStream_t>(stream));
 }
 
-int ugdr_x_expert_ffn_backward(const ugdr_x_experts *m, const void *dy, const void *x, const void *h, const void *gu,
+int ugdr_x_expert_ffn_backward(const ugdr_x_experts *m, const void *dy, const void *x, const void *h, const float *gu,
                                void *dgu, void *dx, void *dw_in, void *dw_out, void *stream) {
     if (!valid(m) || !aligned16(dw_in) || !aligned16(dw_out)) return int(cudaErrorInvalidValue);
     const auto s = static_cast<cudaStream_t>(stream);

@@ -9,8 +9,8 @@
 
 namespace ugdr::coll {
 
-int launch_expert_ffn(const ugdr_x_experts &m, const void *x, void *y, void *h, void *gu, cudaStream_t s);
-int launch_expert_ffn_backward(const ugdr_x_experts &m, const void *dy, const void *x, const void *h, const void *gu,
+int launch_expert_ffn(const ugdr_x_experts &m, const void *x, void *y, void *h, float *gu, cudaStream_t s);
+int launch_expert_ffn_backward(const ugdr_x_experts &m, const void *dy, const void *x, const void *h, const float *gu,
                                void *dgu, void *dx, void *dw_in, void *dw_out, cudaStream_t s);
 
 // A plan in memory: n tensors, then n + 1 first-chunk indices.

@@ -45,15 +45,15 @@ typedef struct ugdr_x_experts {
 } ugdr_x_experts;
 
 /* Forward: g = x Wg^T, u = x Wu^T, h = a(g) * u, y = h Wo^T.  `h` ([rows][inner]) is scratch of a
- * serving call; with `gu` ([rows][2][inner], may be NULL) g and u are kept too, and h and gu are
- * what the backward pass takes.  y may be x itself (the products with x are over by then). */
-int ugdr_x_expert_ffn(const ugdr_x_experts *m, const void *x, void *y, void *h, void *gu, void *stream);
+ * serving call; with `gu` ([rows][2][inner] floats, may be NULL) g and u are kept too, and h and gu
+ * are what the backward pass takes.  y may be x itself (the products with x are over by then). */
+int ugdr_x_expert_ffn(const ugdr_x_experts *m, const void *x, void *y, void *h, float *gu, void *stream);
 
 /* Backward of y with respect to x and the weights, from dy and what the forward pass kept:
  * dh = dy Wo, dg = dh * u * a'(g), du = dh * a(g), dx = dg Wg + du Wu, dw_in = (dg^T x, du^T x),
  * dw_out = dy^T h.  The gradients of an expert without rows are zeros.  `dgu` ([rows][2][inner]) is
  * scratch.  dx may be x or dy itself; the other outputs overlap nothing. */
-int ugdr_x_expert_ffn_backward(const ugdr_x_experts *m, const void *dy, const void *x, const void *h, const void *gu,
+int ugdr_x_expert_ffn_backward(const ugdr_x_experts *m, const void *dy, const void *x, const void *h, const float *gu,
                                void *dgu, void *dx, void *dw_in, void *dw_out, void *stream);
 
 /* One gradient tensor of a plan: `count` elements of `grad_type` at `grad`, scaled into `out`

@@ -1,7 +1,7 @@
 """The experts' gated feed-forward block, forward and backward, against its formulas in fp64.
 
-Tolerances are bounds, element by element, derived from what the operator rounds: h, g, u, dg and
-du once to the type (half a step: eps / 2 of the value, or half the smallest subnormal), the output
+Tolerances are bounds, element by element, derived from what the operator rounds: h, dg and du
+once to the type (half a step: eps / 2 of the value, or half the smallest subnormal), the output
 once, and fp32 sums of n products, off by at most n * 2^-23 of the sum of the products' sizes
 (either way of rounding an addition)."""
 from __future__ import annotations
@@ -59,7 +59,6 @@ def oracle(x, w_in, w_out, act, dy=None):
     dy = dy.double()
     dh = dy @ w_out
     edh = H * step * (dy.abs() @ w_out.abs())
-    eg, eu = eg + rounding(g.abs() + eg, dtype), eu + rounding(u.abs() + eu, dtype)
     dg, du = dh * u * da, dh * a
     edg = edh * (u.abs() + eu) * 1.13 + dh.abs() * (eu * (da.abs() + 0.8 * eg) + u.abs() * 0.8 * eg)
     edu = edh * (a.abs() + 1.13 * eg) + dh.abs() * 1.13 * eg

@@ -43,10 +43,10 @@ class _Experts(C.Structure):
 
 
 class ExpertFFNSaved(NamedTuple):
-    """What a training forward pass keeps for `expert_ffn_backward` (2 * 3 * rows * inner bytes)."""
+    """What a training forward pass keeps for `expert_ffn_backward` (10 * rows * inner bytes)."""
 
     h: torch.Tensor   # [rows, inner]
-    gu: torch.Tensor  # [rows, 2, inner]
+    gu: torch.Tensor  # [rows, 2, inner] float32: both projections
 
 
 _status: dict[int, torch.Tensor] = {}
@@ -102,9 +102,10 @@ def check_status(device: torch.device | int | None = None) -> None:
                             2: "expert counts are negative or exceed the rows"}.get(st, f"status {st}"))
 
 
-def _rows(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor) -> None:
-    if not isinstance(t, torch.Tensor) or t.device != like.device or t.dtype != like.dtype:
-        raise ValueError(f"{name} must be a {like.dtype} tensor on {like.device}")
+def _rows(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor, dtype: torch.dtype | None = None) -> None:
+    dtype = dtype or like.dtype
+    if not isinstance(t, torch.Tensor) or t.device != like.device or t.dtype != dtype:
+        raise ValueError(f"{name} must be a {dtype} tensor on {like.device}")
     if tuple(t.shape) != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
     if not t.is_contiguous() or t.data_ptr() % 16:
@@ -159,7 +160,7 @@ def _forward(x, counts, w_in, w_out, act, out, stream, train):
         word = _status_word(x.device)
         y = torch.empty_like(x) if out is None else out
         h = torch.empty(m.rows, m.inner, dtype=x.dtype, device=x.device)
-        gu = torch.empty(m.rows, 2, m.inner, dtype=x.dtype, device=x.device) if train else None
+        gu = torch.empty(m.rows, 2, m.inner, dtype=torch.float32, device=x.device) if train else None
         m.status = word.data_ptr()
         check(_lib().ugdr_x_expert_ffn(C.byref(m), x.data_ptr(), y.data_ptr(), h.data_ptr(),
                                        gu.data_ptr() if train else None, s), "ugdr_x_expert_ffn")
@@ -192,7 +193,7 @@ def expert_ffn_backward(dy: torch.Tensor, x: torch.Tensor, counts: torch.Tensor,
     m = _checked(x, counts, w_in, w_out, act)
     _rows(dy, "dy", tuple(x.shape), x)
     _rows(saved.h, "saved.h", (m.rows, m.inner), x)
-    _rows(saved.gu, "saved.gu", (m.rows, 2, m.inner), x)
+    _rows(saved.gu, "saved.gu", (m.rows, 2, m.inner), x, torch.float32)
     inputs = {"dy": dy, "x": x, "counts": counts, "w_in": w_in, "w_out": w_out, "saved.h": saved.h,
               "saved.gu": saved.gu}
     for name, t, like in (("dx", dx, x), ("dw_in", dw_in, w_in), ("dw_out", dw_out, w_out)):
