@@ -550,26 +550,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             } else {
                 // 32 rows at a time, turned around in shared memory: then 4 lanes hold a row's
                 // features, 8 next to each other per lane.
+                const int r = quarter * 8 + lane / 4;
                 for (int c = 0; c < t.rows; c += 32, ++chunk) {
+                    const int64_t row = t.first + c + r;
+                    [[maybe_unused]] float g[4][8], u[4][8];
+                    if constexpr (P == kBack) {  // under way while the accumulators are turned around
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int f = feature + i * 32 + lane % 4 * 8;
+                            if (c + r < t.rows && f < m.inner) {
+                                load8(gu + row * 2 * m.inner + f, g[i]);
+                                load8(gu + row * 2 * m.inner + m.inner + f, u[i]);
+                            }
+                        }
+                    }
                     float v[32];
                     tmem_load(columns + c, v);
                     float *buffer = staging + (chunk & 1) * (kStagingBytes / 4);
 #pragma unroll
                     for (int j = 0; j < 32; ++j) buffer[j * kStagingRow + quarter * 32 + lane] = v[j];
                     epilogue_sync();
-                    const int r = quarter * 8 + lane / 4;
-                    const float *from = buffer + r * kStagingRow;
+                    const float *from = buffer + r * kStagingRow + lane % 4 * 8;
                     if (c + r < t.rows) {
-                        const int64_t row = t.first + c + r;
-                        constexpr int kFeatures = P == kUp ? 64 : 128;
 #pragma unroll
-                        for (int i = lane % 4 * 8; i < kFeatures; i += 32) {
-                            const int f = feature + i;
-                            float a[8], b[8], w[8];
-                            load8(from + i, a);
+                        for (int i = 0; i < (P == kUp ? 2 : 4); ++i) {
+                            const int f = feature + i * 32 + lane % 4 * 8;
+                            [[maybe_unused]] float a[8], b[8], w[8];
+                            load8(from + i * 32, a);
                             if constexpr (P == kUp) {
                                 if (f >= m.inner) break;
-                                load8(from + 64 + i, b);
+                                load8(from + 64 + i * 32, b);
                                 if (gu != nullptr) {
                                     store8(gu + row * 2 * m.inner + f, a);
                                     store8(gu + row * 2 * m.inner + m.inner + f, b);
@@ -579,13 +589,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                 store8(out + row * m.inner + f, w);
                             } else if constexpr (P == kBack) {
                                 if (f >= m.inner) break;
-                                float g[8], u[8];
-                                load8(gu + row * 2 * m.inner + f, g);
-                                load8(gu + row * 2 * m.inner + m.inner + f, u);
 #pragma unroll
                                 for (int j = 0; j < 8; ++j) {
-                                    w[j] = a[j] * u[j] * act_grad(g[j], m.act);
-                                    b[j] = a[j] * act(g[j], m.act);
+                                    w[j] = a[j] * u[i][j] * act_grad(g[i][j], m.act);
+                                    b[j] = a[j] * act(g[i][j], m.act);
                                 }
                                 store8(out + row * 2 * m.inner + f, w);
                                 store8(out + row * 2 * m.inner + m.inner + f, b);

@@ -22,7 +22,7 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kGroup = 8;    // elements a thread takes at once: 16 or 32 bytes
-constexpr int kUnroll = 4;   // groups in flight per thread
+constexpr int kInFlight = 16;  // 16 / element size groups in flight per thread: 128 bytes
 static_assert(kThreads * kGroup == kGradChunk, "one group per thread and chunk");
 
 template <int TYPE> struct Element;
@@ -75,6 +75,13 @@ template <typename T> __device__ __forceinline__ void store_group(T *p, const Gr
                      : "memory");
 }
 
+template <typename O, typename T> __device__ __forceinline__ Group<O> scaled(const Group<T> &g, float coef) {
+    Group<O> o;
+#pragma unroll
+    for (int j = 0; j < kGroup; ++j) from_float(o.v[j], to_float(g.v[j]) * coef);
+    return o;
+}
+
 // The tensor list of a plan: the tensors and the chunk that each begins with.
 struct Plan {
     const ugdr_x_grad *grads;
@@ -103,18 +110,31 @@ __device__ double block_sum(double v) {
     return v;
 }
 
-__device__ __forceinline__ double squares(const float (&f)[kGroup]) {
-    float s = 0.f, most = 0.f;
+template <typename T> __device__ __forceinline__ float squares(const Group<T> &g) {
+    float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < kGroup; ++j) {
-        s = fmaf(f[j], f[j], s);
-        most = fmaxf(most, fabsf(f[j]));
+    for (int j = 0; j < kGroup; ++j) s = fmaf(to_float(g.v[j]), to_float(g.v[j]), s);
+    return s;
+}
+// Whether a group's fp32 sum of squares says less than it should: numbers whose squares fp32 cannot
+// hold (or nothing but zeros).
+__device__ __forceinline__ bool unsafe(float s) { return !(s < 3e38f && s > 1e-30f); }
+__device__ __forceinline__ double squares_wide(float a, double sum) { return fma(double(a), double(a), sum); }
+
+// The squares of `n` groups of one thread, a chunk apart.
+template <typename T> __device__ __noinline__ double squares_wide(const T *p, int n) {
+    double sum = 0;
+#pragma unroll 1
+    for (int u = 0; u < n; ++u, p += kGradChunk) {
+        const Group<T> g = load_group(p);
+        float any = 0;
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) any += fabsf(to_float(g.v[j]));
+        if (any == 0.f) continue;
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) sum = squares_wide(to_float(g.v[j]), sum);
     }
-    if (s < 3e38f && (s > 1e-30f || most == 0.f)) return s;
-    double d = 0;
-#pragma unroll
-    for (int j = 0; j < kGroup; ++j) d = fma(double(f[j]), double(f[j]), d);
-    return d;
+    return sum;
 }
 
 // Elements before the tensor's first that make its base a multiple of a group's bytes: chunk c
@@ -124,33 +144,55 @@ template <typename T> __device__ __forceinline__ uint32_t lead_of(const T *p) {
     return uint32_t(reinterpret_cast<uintptr_t>(p) % (sizeof(T) * kGroup) / sizeof(T));
 }
 
+// The chunks of [c0, c1) that lie in the tensor as a whole: [whole.a, whole.b).  At most the first
+// and the last do not.
+struct Whole {
+    uint32_t a, b;
+};
+__device__ __forceinline__ Whole whole_chunks(uint32_t c0, uint32_t c1, uint32_t lead, uint64_t n) {
+    const uint32_t a = c0 == 0 && lead != 0 ? 1 : c0;
+    const uint32_t b = uint32_t(min(uint64_t(c1), (n + lead) / kGradChunk));
+    return {min(a, c1), max(min(a, c1), b)};
+}
+
 // The squares of the chunks [c0, c1) of one tensor.
 template <int TYPE> __device__ double span_squares(const ugdr_x_grad &t, uint32_t c0, uint32_t c1) {
     using T = typename Element<TYPE>::type;
+    constexpr int kUnroll = kInFlight / sizeof(T);
     const T *g = static_cast<const T *>(t.grad);
-    const int64_t lead = lead_of(g), n = int64_t(t.count);
+    const uint32_t lead = lead_of(g);
+    const int64_t n = int64_t(t.count);
+    const Whole w = whole_chunks(c0, c1, lead, t.count);
+    const T *p = g + (int64_t(w.a) * kGradChunk + threadIdx.x * kGroup - int64_t(lead));
     double acc = 0;
-    for (uint32_t c = c0; c < c1; c += kUnroll) {
+    uint32_t c = w.a;
+    for (; c + kUnroll <= w.b; c += kUnroll, p += kUnroll * kGradChunk) {
         Group<T> v[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int64_t at = int64_t(c + u) * kGradChunk + threadIdx.x * kGroup - lead;
-            if (c + u < c1 && at >= 0 && at + kGroup <= n) {
-                v[u] = load_group(g + at);
-            } else {
+        for (int u = 0; u < kUnroll; ++u) v[u] = load_group(p + u * kGradChunk);
+        double sum = 0;
+        bool wide = false;
 #pragma unroll
-                for (int j = 0; j < kGroup; ++j) {
-                    from_float(v[u].v[j], 0.f);
-                    if (c + u < c1 && at + j >= 0 && at + j < n) v[u].v[j] = g[at + j];
-                }
-            }
+        for (int u = 0; u < kUnroll; ++u) {
+            const float q = squares(v[u]);
+            wide |= unsafe(q);
+            sum += double(q);
         }
+        acc += wide ? squares_wide(p, kUnroll) : sum;
+    }
+    for (; c < w.b; ++c, p += kGradChunk) {
+        const float q = squares(load_group(p));
+        acc += unsafe(q) ? squares_wide(p, 1) : double(q);
+    }
+    for (uint32_t edge = c0; edge < c1; ++edge) {
+        if (edge == w.a && w.a < w.b) edge = w.b;
+        if (edge == c1) break;
+        // Neighbours to neighbouring threads, and every square in fp64.
+        const int64_t at = int64_t(edge) * kGradChunk - int64_t(lead) + threadIdx.x;
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            float f[kGroup];
-#pragma unroll
-            for (int j = 0; j < kGroup; ++j) f[j] = to_float(v[u].v[j]);
-            acc += squares(f);
+        for (int j = 0; j < kGroup; ++j) {
+            const int64_t i = at + j * kThreads;
+            if (i >= 0 && i < n) acc = squares_wide(to_float(g[i]), acc);
         }
     }
     return acc;
@@ -197,36 +239,40 @@ __global__ void __launch_bounds__(kThreads) grad_sum_kernel(const double *partia
 template <int IN, int OUT> __device__ void span_scale(const ugdr_x_grad &t, uint32_t c0, uint32_t c1, float coef) {
     using T = typename Element<IN>::type;
     using O = typename Element<OUT>::type;
+    constexpr int kUnroll = 4;
     const T *g = static_cast<const T *>(t.grad);
     O *out = static_cast<O *>(t.out);
-    const int64_t lead = lead_of(g), n = int64_t(t.count);
-    const bool whole = lead_of(out) == uint32_t(lead);  // whole groups of the output are aligned too
-    for (uint32_t left = c1 - c0; left > 0; left -= min(left, uint32_t(kUnroll))) {
+    const uint32_t lead = lead_of(g);
+    const int64_t n = int64_t(t.count), mine = int64_t(threadIdx.x * kGroup) - int64_t(lead);
+    Whole w = whole_chunks(c0, c1, lead, t.count);
+    if (lead_of(out) != lead) w.b = w.a;  // whole groups of the output are not aligned
+    for (uint32_t edge = c0; edge < c1; ++edge) {
+        if (edge == w.a && w.a < w.b) edge = w.b;
+        if (edge == c1) break;
+        // Neighbours to neighbouring threads.
+        const int64_t at = int64_t(edge) * kGradChunk - int64_t(lead) + threadIdx.x;
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) {
+            const int64_t i = at + j * kThreads;
+            if (i >= 0 && i < n) from_float(out[i], to_float(g[i]) * coef);
+        }
+    }
+    const T *p = g + (int64_t(w.b) * kGradChunk + mine);
+    O *o = out + (int64_t(w.b) * kGradChunk + mine);
+    uint32_t left = w.b - w.a;
+    for (; left >= kUnroll; left -= kUnroll) {
         Group<T> v[kUnroll];
+        p -= kUnroll * kGradChunk;
+        o -= kUnroll * kGradChunk;
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int64_t at = (int64_t(c0) + left - 1 - u) * kGradChunk + threadIdx.x * kGroup - lead;
-            if (uint32_t(u) < left && at >= 0 && at + kGroup <= n) v[u] = load_group(g + at);
-        }
+        for (int u = 0; u < kUnroll; ++u) v[u] = load_group(p + u * kGradChunk);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            if (uint32_t(u) >= left) break;
-            const int64_t at = (int64_t(c0) + left - 1 - u) * kGradChunk + threadIdx.x * kGroup - lead;
-            if (at >= 0 && at + kGroup <= n) {
-                Group<O> o;
-#pragma unroll
-                for (int j = 0; j < kGroup; ++j) from_float(o.v[j], to_float(v[u].v[j]) * coef);
-                if (whole) {
-                    store_group(out + at, o);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < kGroup; ++j) out[at + j] = o.v[j];
-                }
-            } else {
-                for (int j = 0; j < kGroup; ++j)
-                    if (at + j >= 0 && at + j < n) from_float(out[at + j], to_float(g[at + j]) * coef);
-            }
-        }
+        for (int u = 0; u < kUnroll; ++u) store_group(o + u * kGradChunk, scaled<O>(v[u], coef));
+    }
+    for (; left > 0; --left) {
+        p -= kGradChunk;
+        o -= kGradChunk;
+        store_group(o, scaled<O>(load_group(p), coef));
     }
 }
 
