@@ -18,7 +18,7 @@
 //   Rows that follow the group in the last 64-deep step must not count, whatever they hold: a
 //   warp overwrites them with zeros in shared memory, up to the 16 that one instruction takes.
 // * Warp 0 issues the TMA loads into a ring of stages, warp 1 of the leading CTA the matrix
-//   instructions, warp 2 clears tails, warps 4 to 7 move finished accumulators out of TMEM, where
+//   instructions, warp 2 clears tails, warps 4 to 11 move finished accumulators out of TMEM, where
 //   two tiles' accumulators fit, so that they overlap the next tile's products.
 // * Every pair walks the tile list by itself (tile t, t + pairs, ...): the row counts are read on
 //   the device, and no CTA waits for another outside its pair.
@@ -40,7 +40,7 @@
 namespace ugdr::coll {
 namespace {
 
-constexpr int kThreads = 256;       // 8 warps
+constexpr int kThreads = 384;       // 12 warps: 4 that feed the tensor cores, 8 for the epilogue
 constexpr int kHalf = 128;          // features of a tile per CTA: the lanes of TMEM
 constexpr int kPairFeatures = 256;
 constexpr int kMaxN = 256;
@@ -199,14 +199,15 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
                  : "r"(addr)
                  : "memory");
 }
-__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-// Whether all four epilogue warps say so: one that gives up takes the others along.
-__device__ __forceinline__ bool epilogue_all(bool ok) {
+// The four warps of an epilogue group, 0 or 1, meet.
+__device__ __forceinline__ void group_sync(int group) { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); }
+// Whether all of them say so: one that gives up takes the others along.
+__device__ __forceinline__ bool group_all(int group, bool ok) {
     uint32_t all;
     asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\n"
-                 "bar.red.and.pred q, 1, 128, p;\nselp.u32 %0, 1, 0, q;\n}"
+                 "bar.red.and.pred q, %2, 128, p;\nselp.u32 %0, 1, 0, q;\n}"
                  : "=r"(all)
-                 : "r"(uint32_t(ok))
+                 : "r"(uint32_t(ok)), "r"(1 + group)
                  : "memory");
     return all != 0;
 }
@@ -332,17 +333,18 @@ __device__ __forceinline__ void load8(const float *p, float *v) {
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
-// The activation and its derivative.
-__device__ __forceinline__ float act(float g, int kind) {
-    if (kind == UGDR_X_ACT_SILU) return g / (1.f + expf(-g));
-    return 0.5f * g * (1.f + erff(g * 0.70710678f));
+// a(g) and a'(g).  The reciprocal is the approximate one (1 ulp): 1 + exp(-g) is between 1 and
+// infinity, whose reciprocal is the 0 that belongs there.
+struct Act {
+    float a, da;
+};
+__device__ __forceinline__ Act silu(float g) {
+    const float s = __fdividef(1.f, 1.f + expf(-g));
+    return {g * s, s * (1.f + g * (1.f - s))};
 }
-__device__ __forceinline__ float act_grad(float g, int kind) {
-    if (kind == UGDR_X_ACT_SILU) {
-        const float s = 1.f / (1.f + expf(-g));
-        return s * (1.f + g * (1.f - s));
-    }
-    return 0.5f * (1.f + erff(g * 0.70710678f)) + g * 0.39894228f * expf(-0.5f * g * g);
+__device__ __forceinline__ Act gelu(float g) {
+    const float p = 0.5f + 0.5f * erff(g * 0.70710678f);
+    return {g * p, p + g * 0.39894228f * expf(-0.5f * g * g)};
 }
 
 // ---- the kernel --------------------------------------------------------------------------------
@@ -374,7 +376,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(smem_addr(&sh.tmem_full[s]), 1);
-            mbar_init(smem_addr(&sh.tmem_empty[s]), 8);  // 4 epilogue warps of each CTA
+            mbar_init(smem_addr(&sh.tmem_empty[s]), 16);  // 8 epilogue warps of each CTA
         }
         sh.aborted = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -514,16 +516,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             __syncwarp();
         }
     } else if (warp >= 4) {
-        // Finished accumulators.  This warp's TMEM lanes are features 32 (warp % 4) ... + 31.
-        const int quarter = warp % 4;
+        // Finished accumulators.  This warp's TMEM lanes are features 32 (warp % 4) ... + 31; its
+        // group of four warps takes every other 32 columns.
+        const int quarter = warp % 4, group = warp / 4 - 1;
         const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
         Tiles<P> tiles(m, first);
         Tile t;
-        uint32_t acc = 0, chunk = 0;
+        uint32_t acc = 0;
         for (int at = pair; tiles.next(at, t); at += pairs) {
             const bool none = steps_of<P>(m, t) == 0;
             if (!none) {
-                if (!epilogue_all(mbar_wait(smem_addr(&sh.tmem_full[acc & 1]), (acc / 2) & 1, sh, m.status))) break;
+                if (!group_all(group, mbar_wait(smem_addr(&sh.tmem_full[acc & 1]), (acc / 2) & 1, sh, m.status)))
+                    break;
                 fence_after();
             }
             const uint32_t columns = lanes + (acc & 1) * kMaxN;
@@ -533,7 +537,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int width = P == kGradOut ? m.inner : m.hidden, height = P == kGradOut ? m.hidden : m.inner;
                 const int f = feature + quarter * 32 + lane;
                 T *row = out + ((int64_t(t.expert) * (P == kGradIn ? 2 : 1) + t.part) * height + f) * width + t.column;
-                for (int c = 0; c < kMaxN; c += 32) {
+                for (int c = group * 32; c < kMaxN; c += 64) {
                     float v[32];
                     if (none) {
 #pragma unroll
@@ -551,7 +555,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 // 32 rows at a time, turned around in shared memory: then 4 lanes hold a row's
                 // features, 8 next to each other per lane.
                 const int r = quarter * 8 + lane / 4;
-                for (int c = 0; c < t.rows; c += 32, ++chunk) {
+                for (int c = group * 32; c < t.rows; c += 64) {
                     const int64_t row = t.first + c + r;
                     [[maybe_unused]] float g[4][8], u[4][8];
                     if constexpr (P == kBack) {  // under way while the accumulators are turned around
@@ -566,10 +570,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
                     float v[32];
                     tmem_load(columns + c, v);
-                    float *buffer = staging + (chunk & 1) * (kStagingBytes / 4);
+                    float *buffer = staging + group * (kStagingBytes / 4);
 #pragma unroll
                     for (int j = 0; j < 32; ++j) buffer[j * kStagingRow + quarter * 32 + lane] = v[j];
-                    epilogue_sync();
+                    group_sync(group);
                     const float *from = buffer + r * kStagingRow + lane % 4 * 8;
                     if (c + r < t.rows) {
 #pragma unroll
@@ -584,15 +588,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                     store8(gu + row * 2 * m.inner + f, a);
                                     store8(gu + row * 2 * m.inner + m.inner + f, b);
                                 }
+                                if (m.act == UGDR_X_ACT_SILU) {
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) w[j] = act(a[j], m.act) * b[j];
+                                    for (int j = 0; j < 8; ++j) w[j] = silu(a[j]).a * b[j];
+                                } else {
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j) w[j] = gelu(a[j]).a * b[j];
+                                }
                                 store8(out + row * m.inner + f, w);
                             } else if constexpr (P == kBack) {
                                 if (f >= m.inner) break;
+                                if (m.act == UGDR_X_ACT_SILU) {
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    w[j] = a[j] * u[i][j] * act_grad(g[i][j], m.act);
-                                    b[j] = a[j] * act(g[i][j], m.act);
+                                    for (int j = 0; j < 8; ++j) {
+                                        const Act s = silu(g[i][j]);
+                                        w[j] = a[j] * u[i][j] * s.da;
+                                        b[j] = a[j] * s.a;
+                                    }
+                                } else {
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j) {
+                                        const Act s = gelu(g[i][j]);
+                                        w[j] = a[j] * u[i][j] * s.da;
+                                        b[j] = a[j] * s.a;
+                                    }
                                 }
                                 store8(out + row * 2 * m.inner + f, w);
                                 store8(out + row * 2 * m.inner + m.inner + f, b);
@@ -602,6 +621,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             }
                         }
                     }
+                    group_sync(group);  // the buffer is free again
                 }
             }
             if (!none) {
