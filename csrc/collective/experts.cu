@@ -35,6 +35,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <type_traits>
 
 namespace ugdr::coll {
@@ -46,7 +47,7 @@ constexpr int kPairFeatures = 256;
 constexpr int kMaxN = 256;
 constexpr int kStepN = 32;
 constexpr int kDepth = 64;          // elements per stage along the summed dimension: 128 bytes
-constexpr int kSmallBox = 16;       // rows of the small TMA box: half of kStepN
+constexpr int kBoxes = 4;            // TMA boxes of 128, 64, 32 and 16 rows
 constexpr int kStages = 5;
 constexpr int kBand = 8;            // row tiles that run through all features before the next
 constexpr uint32_t kOperandBytes = kHalf * kDepth * 2;  // one CTA's half of A, or of B, in a stage
@@ -181,6 +182,10 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
                  "h"(uint16_t(3))
                  : "memory");
 }
+// Programmatic launches: the next kernel of the stream may begin its set-up, and this one waits here
+// until the kernels before it are over and their writes visible.
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
@@ -349,8 +354,11 @@ __device__ __forceinline__ Act gelu(float g) {
 
 // ---- the kernel --------------------------------------------------------------------------------
 
+// B's boxes: half of the N rows, rounded up to 32, is a sum of at most two of 128, 64 and 32, and
+// the smallest half has one of 16.  With boxes of 16 rows only, 224 rows per expert took longer than
+// 256; with 32 at least, single rows per expert read their weights at 5.6 TB/s instead of 6.3.
 struct Maps {
-    CUtensorMap a, b, b_small;
+    CUtensorMap a, b[kBoxes];
 };
 
 template <typename T, Product P>
@@ -368,6 +376,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t stage0 = smem_addr(tiles_mem);
     constexpr bool kInnerA = kFeaturesInner<P>, kInnerB = kWeightGrad<P>;
 
+    launch_next();
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(smem_addr(&sh.full[s]), 2);   // both CTAs' loads, counted in the leading CTA
@@ -381,12 +390,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         sh.aborted = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    scan_counts(m, sh, first);
     if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sh.tmem))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
+    if (threadIdx.x >= 32 && threadIdx.x < 32 + 1 + (kWeightGrad<P> ? 1 : kBoxes))
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a + (threadIdx.x - 32)) : "memory");
+    wait_previous();
+    scan_counts(m, sh, first);
     fence_before();
     __syncthreads();
     cluster_sync();
@@ -401,8 +413,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         bool go = true;
         for (int at = pair; go && tiles.next(at, t); at += pairs) {
             const int steps = steps_of<P>(m, t), n = ceil_div(t.rows, kStepN) * kStepN;
-            const int half = kWeightGrad<P> ? kHalf : n / 2;
-            const uint32_t bytes = kOperandBytes + uint32_t(half) * kDepth * 2;
+            const int half = kWeightGrad<P> ? kHalf : n / 2, load = half == 16 ? half : ceil_div(half, 32) * 32;
+            const uint32_t bytes = kOperandBytes + uint32_t(load) * kDepth * 2;
             const int feature = t.feature + int(rank) * (kTileFeatures<P> / 2);
             for (int k = 0; k < steps; ++k, ++it) {
                 const uint32_t s = it % kStages;
@@ -439,20 +451,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
                 if constexpr (kWeightGrad<P>) {
                     for (int c = 0; c < 2; ++c)
-                        tma_load(b + uint32_t(c) * kOperandBytes / 2, &maps.b, bar,
+                        tma_load(b + uint32_t(c) * kOperandBytes / 2, &maps.b[0], bar,
                                  t.column + int(rank) * kHalf + c * 64, t.first + depth);
                 } else {
-                    const bool whole = half == kHalf;
-                    const int box = whole ? kHalf : kSmallBox, row = t.first + int(rank) * half;
-                    const CUtensorMap *map = whole ? &maps.b : &maps.b_small;
-                    for (int r = 0; r < half; r += box) {
+                    for (int r = 0, box = kHalf, i = 0; r < load; box /= 2, ++i) {
+                        if (load - r < box) continue;
                         const uint32_t dst = b + uint32_t(r) * kDepth * 2;
+                        const int row = t.first + int(rank) * half + r;
                         if constexpr (P == kInput) {
                             const int part = k >= steps / 2;
-                            tma_load(dst, map, bar, depth - part * (steps / 2) * kDepth, part, row + r);
+                            tma_load(dst, &maps.b[i], bar, depth - part * (steps / 2) * kDepth, part, row);
                         } else {
-                            tma_load(dst, map, bar, depth, row + r);
+                            tma_load(dst, &maps.b[i], bar, depth, row);
                         }
+                        r += box;
                     }
                 }
             }
@@ -683,6 +695,25 @@ template <typename T> bool encode(CUtensorMap *map, const Dense &d) {
                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Once per kernel and device: its shared memory.  The device's SM count in *sms.
+cudaError_t set_up(const void *kernel, int device, int index, int *sms) {
+    constexpr int kDevices = 64;
+    static std::atomic<int> known_sms[kDevices];
+    static std::atomic<uint32_t> done[kDevices];
+    const bool kept = device < kDevices;
+    *sms = kept ? known_sms[device].load(std::memory_order_relaxed) : 0;
+    if (*sms == 0) {
+        if (cudaError_t e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device); e != cudaSuccess)
+            return e;
+        if (kept) known_sms[device].store(*sms, std::memory_order_relaxed);
+    }
+    if (kept && (done[device].load(std::memory_order_relaxed) >> index & 1)) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               int(shared_bytes(UGDR_X_EXPERTS_MAX)));
+    if (e == cudaSuccess && kept) done[device].fetch_or(1u << index, std::memory_order_relaxed);
+    return e;
+}
+
 // One product.  `a` and `b` are its operands: the weights and the rows, or the two row tensors of a
 // weight gradient.
 template <typename T, Product P>
@@ -701,28 +732,35 @@ cudaError_t launch(const ugdr_x_experts &m, const void *a, const void *b, void *
         da = {a, 2, {H, R}, {64, 64}};
     else
         da = {a, 3, {F, 2, R}, {64, 1, 64}};
-    const cuuint32_t rows = kWeightGrad<P> ? 64 : kHalf;
     if (P == kInput)
-        db = {b, 3, {F, 2, R}, {64, 1, rows}};
+        db = {b, 3, {F, 2, R}, {64, 1, 0}};
     else
-        db = {b, 2, {P == kUp || P == kBack || P == kGradIn ? H : F, R}, {64, rows}};
+        db = {b, 2, {P == kUp || P == kBack || P == kGradIn ? H : F, R}, {64, 0}};
     Maps maps;
-    if (!encode<T>(&maps.a, da) || !encode<T>(&maps.b, db)) return cudaErrorInvalidValue;
-    db.box[db.rank - 1] = kSmallBox;
-    if (!encode<T>(&maps.b_small, db)) return cudaErrorInvalidValue;
+    if (!encode<T>(&maps.a, da)) return cudaErrorInvalidValue;
+    for (int i = 0; i < (kWeightGrad<P> ? 1 : kBoxes); ++i) {
+        db.box[db.rank - 1] = kWeightGrad<P> ? kDepth : kHalf >> i;
+        if (!encode<T>(&maps.b[i], db)) return cudaErrorInvalidValue;
+    }
 
+    auto *kernel = expert_kernel<T, P>;
     int device = 0, sms = 0;
     if (cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return e;
-    if (cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device); e != cudaSuccess) return e;
-    const size_t bytes = shared_bytes(m.nexp);
-    auto *kernel = expert_kernel<T, P>;
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             int(shared_bytes(UGDR_X_EXPERTS_MAX)));
+    if (cudaError_t e = set_up(reinterpret_cast<const void *>(kernel), device, int(P) * 2 + std::is_same_v<T, __half>, &sms);
         e != cudaSuccess)
         return e;
+    cudaLaunchAttribute programmatic{};
+    programmatic.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    programmatic.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(unsigned(sms / 2 * 2));
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = shared_bytes(m.nexp);
+    config.stream = s;
+    config.attrs = &programmatic;
+    config.numAttrs = 1;
     const Shape shape{m.counts, m.status, int(m.rows), m.nexp, m.hidden, m.inner, m.act};
-    kernel<<<sms / 2 * 2, kThreads, bytes, s>>>(maps, shape, static_cast<T *>(out), gu);
-    return cudaGetLastError();
+    return cudaLaunchKernelEx(&config, kernel, maps, shape, static_cast<T *>(out), gu);
 }
 
 template <typename T>

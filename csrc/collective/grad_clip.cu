@@ -203,6 +203,7 @@ __device__ __forceinline__ uint32_t share(uint32_t chunks, uint32_t block) {
 }
 
 __global__ void __launch_bounds__(kThreads, 2) grad_norm_kernel(Plan p, uint32_t chunks, double *partials) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t c1 = share(chunks, blockIdx.x + 1);
     uint32_t c = share(chunks, blockIdx.x);
     double acc = 0;
@@ -280,6 +281,7 @@ template <int IN, int OUT> __device__ void span_scale(const ugdr_x_grad &t, uint
 // scales its run of chunks backwards: what the norm pass read last is what the L2 still holds.
 __global__ void __launch_bounds__(kThreads, 2) grad_scale_kernel(Plan p, uint32_t chunks, const double *partials,
                                                                  int npartials, float max_norm, float *norm_out) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the norm kernel's sums are there
     const double norm = sqrt(partial_sum(partials, npartials));
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = float(norm);
     const double ratio = double(max_norm) / (norm + 1e-6);
@@ -339,10 +341,20 @@ int launch_grad_clip(const void *plan, int n, uint64_t chunks, double *partials,
     const int blocks = blocks_for(chunks);
     if (sum_squares == nullptr)
         grad_norm_kernel<<<blocks, kThreads, 0, s>>>(as_plan(plan, n), uint32_t(chunks), partials);
-    grad_scale_kernel<<<blocks, kThreads, 0, s>>>(as_plan(plan, n), uint32_t(chunks),
-                                                  sum_squares == nullptr ? partials : sum_squares,
-                                                  sum_squares == nullptr ? blocks : 1, max_norm, norm_out);
-    return int(cudaGetLastError());
+    // Launched while the norm kernel runs: its blocks start as those of the norm kernel end.
+    cudaLaunchAttribute programmatic{};
+    programmatic.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    programmatic.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(unsigned(blocks));
+    config.blockDim = dim3(kThreads);
+    config.stream = s;
+    config.attrs = &programmatic;
+    config.numAttrs = sum_squares == nullptr ? 1 : 0;
+    if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return int(e);
+    return int(cudaLaunchKernelEx(&config, grad_scale_kernel, as_plan(plan, n), uint32_t(chunks),
+                                  static_cast<const double *>(sum_squares == nullptr ? partials : sum_squares),
+                                  sum_squares == nullptr ? blocks : 1, max_norm, norm_out));
 }
 
 }  // namespace ugdr::coll

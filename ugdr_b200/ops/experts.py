@@ -64,17 +64,31 @@ def _lib() -> C.CDLL:
     return L
 
 
-@contextlib.contextmanager
-def _on(device: torch.device, stream: torch.cuda.Stream | None):
-    """The tensors' device current, and `stream` the one that outputs and scratch are allocated for."""
-    if stream is not None and stream.device != device:
-        raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
-    with torch.cuda.device(device):
-        if stream is None:
-            yield torch.cuda.current_stream(device).cuda_stream
-        else:
-            with torch.cuda.stream(stream):
-                yield stream.cuda_stream
+class _On:
+    """The tensors' device current, and `stream` the one that outputs and scratch are allocated for;
+    as a context, the raw stream.  A class, and the raw stream without a Stream object: the calls
+    around it take a few microseconds."""
+
+    __slots__ = ("device", "stream", "guards")
+
+    def __init__(self, device: torch.device, stream: torch.cuda.Stream | None):
+        if stream is not None and stream.device != device:
+            raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+        self.device, self.stream, self.guards = device, stream, None
+
+    def __enter__(self) -> int:
+        if self.stream is None and torch.cuda.current_device() == self.device.index:
+            return torch._C._cuda_getCurrentRawStream(self.device.index)
+        self.guards = contextlib.ExitStack()
+        self.guards.enter_context(torch.cuda.device(self.device))
+        if self.stream is None:
+            return torch._C._cuda_getCurrentRawStream(self.device.index)
+        self.guards.enter_context(torch.cuda.stream(self.stream))
+        return self.stream.cuda_stream
+
+    def __exit__(self, *exc) -> None:
+        if self.guards is not None:
+            self.guards.close()
 
 
 def _status_word(device: torch.device) -> torch.Tensor:
@@ -156,7 +170,7 @@ def _forward(x, counts, w_in, w_out, act, out, stream, train):
     if out is not None:
         _rows(out, "out", tuple(x.shape), x)
         _apart(out, "out", {"x": x, "counts": counts, "w_in": w_in, "w_out": w_out}, () if train else ("x",))
-    with _on(x.device, stream) as s:
+    with _On(x.device, stream) as s:
         word = _status_word(x.device)
         y = torch.empty_like(x) if out is None else out
         h = torch.empty(m.rows, m.inner, dtype=x.dtype, device=x.device)
@@ -201,7 +215,7 @@ def expert_ffn_backward(dy: torch.Tensor, x: torch.Tensor, counts: torch.Tensor,
             _rows(t, name, tuple(like.shape), x)
             _apart(t, name, inputs, ("dy", "x") if name == "dx" else ())
             inputs[name] = t
-    with _on(x.device, stream) as s:
+    with _On(x.device, stream) as s:
         word = _status_word(x.device)
         dx = torch.empty_like(x) if dx is None else dx
         dw_in = torch.empty_like(w_in) if dw_in is None else dw_in

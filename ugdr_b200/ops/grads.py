@@ -15,7 +15,7 @@ import torch
 
 from .. import _native as N
 from ..parallel.peers import check
-from .experts import _on, _overlap
+from .experts import _On, _overlap
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 PARTIALS = 2048
@@ -107,7 +107,7 @@ class GradClip:
 
     def sum_squares(self, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
         """The sum of the squares of all elements, a float64 tensor on the device."""
-        with _on(self.device, stream) as s:
+        with _On(self.device, stream) as s:
             partials = torch.empty(PARTIALS, dtype=torch.float64, device=self.device)
             total = torch.empty((), dtype=torch.float64, device=self.device)
             check(_lib().ugdr_x_grad_sum_squares(self._plan.data_ptr(), self._n, self._chunks, partials.data_ptr(),
@@ -126,7 +126,7 @@ class GradClip:
         if sum_squares is not None and (not isinstance(sum_squares, torch.Tensor) or sum_squares.numel() != 1
                                         or sum_squares.dtype != torch.float64 or sum_squares.device != self.device):
             raise ValueError(f"sum_squares must be one float64 on {self.device}")
-        with _on(self.device, stream) as s:
+        with _On(self.device, stream) as s:
             partials = torch.empty(PARTIALS, dtype=torch.float64, device=self.device)
             norm = torch.empty((), dtype=torch.float32, device=self.device)
             check(_lib().ugdr_x_grad_clip(self._plan.data_ptr(), self._n, self._chunks, partials.data_ptr(),
