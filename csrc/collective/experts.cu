@@ -48,11 +48,12 @@ constexpr int kMaxN = 256;
 constexpr int kStepN = 32;
 constexpr int kDepth = 64;          // elements per stage along the summed dimension: 128 bytes
 constexpr int kBoxes = 4;            // TMA boxes of 128, 64, 32 and 16 rows
-constexpr int kStages = 5;
+constexpr int kStages = 6;
+constexpr int kChunk = 16;          // rows (or columns of a gradient) that an epilogue group moves at once
 constexpr int kBand = 8;            // row tiles that run through all features before the next
 constexpr uint32_t kOperandBytes = kHalf * kDepth * 2;  // one CTA's half of A, or of B, in a stage
 constexpr int kStagingRow = kHalf + 4;                  // floats; the 4 keep 16-byte reads apart
-constexpr uint32_t kStagingBytes = 32 * kStagingRow * 4;
+constexpr uint32_t kStagingBytes = kChunk * kStagingRow * 4;
 constexpr uint64_t kWaitNs = 5ull * 1000 * 1000 * 1000;
 
 enum Product { kUp, kDown, kBack, kInput, kGradOut, kGradIn };
@@ -189,18 +190,15 @@ __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.w
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
-// 32 columns of this warp's 32 TMEM lanes: v[j] is column j of lane threadIdx.x % 32.
-__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
+// 16 columns of this warp's 32 TMEM lanes: v[j] is column j of lane threadIdx.x % 32.
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[kChunk]) {
     uint32_t *r = reinterpret_cast<uint32_t *>(v);
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
                  "tcgen05.wait::ld.sync.aligned;"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
                    "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-                   "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
-                   "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
-                   "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                   "=r"(r[15])
                  : "r"(addr)
                  : "memory");
 }
@@ -553,7 +551,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
     } else if (warp >= 4) {
         // Finished accumulators.  This warp's TMEM lanes are features 32 (warp % 4) ... + 31; its
-        // group of four warps takes every other 32 columns.
+        // group of four warps takes every other chunk of columns.
         const int quarter = warp % 4, group = warp / 4 - 1;
         const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
         Tiles<P> tiles(m, first);
@@ -573,53 +571,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int width = P == kGradOut ? m.inner : m.hidden, height = P == kGradOut ? m.hidden : m.inner;
                 const int f = feature + quarter * 32 + lane;
                 T *row = out + ((int64_t(t.expert) * (P == kGradIn ? 2 : 1) + t.part) * height + f) * width + t.column;
-                for (int c = group * 32; c < kMaxN; c += 64) {
-                    float v[32];
+                for (int c = group * kChunk; c < kMaxN; c += 2 * kChunk) {
+                    float v[kChunk];
                     if (none) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = 0.f;
+                        for (int j = 0; j < kChunk; ++j) v[j] = 0.f;
                     } else {
                         tmem_load(columns + c, v);
                     }
                     if (f < height) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 8)
+                        for (int j = 0; j < kChunk; j += 8)
                             if (t.column + c + j < width) store8(row + c + j, v + j);
                     }
                 }
             } else {
-                // 32 rows at a time, turned around in shared memory: then 4 lanes hold a row's
-                // features, 8 next to each other per lane.
-                const int r = quarter * 8 + lane / 4;
-                for (int c = group * 32; c < t.rows; c += 64) {
+                // A chunk of rows at a time, turned around in shared memory: then 8 lanes hold 64 of a
+                // row's features, 8 next to each other per lane.
+                const int r = quarter * 4 + lane / 8;
+                for (int c = group * kChunk; c < t.rows; c += 2 * kChunk) {
                     const int64_t row = t.first + c + r;
-                    [[maybe_unused]] float g[4][8], u[4][8];
+                    [[maybe_unused]] float g[2][8], u[2][8];
                     if constexpr (P == kBack) {  // under way while the accumulators are turned around
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int f = feature + i * 32 + lane % 4 * 8;
+                        for (int i = 0; i < 2; ++i) {
+                            const int f = feature + i * 64 + lane % 8 * 8;
                             if (c + r < t.rows && f < m.inner) {
                                 load8(gu + row * 2 * m.inner + f, g[i]);
                                 load8(gu + row * 2 * m.inner + m.inner + f, u[i]);
                             }
                         }
                     }
-                    float v[32];
+                    float v[kChunk];
                     tmem_load(columns + c, v);
                     float *buffer = staging + group * (kStagingBytes / 4);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) buffer[j * kStagingRow + quarter * 32 + lane] = v[j];
+                    for (int j = 0; j < kChunk; ++j) buffer[j * kStagingRow + quarter * 32 + lane] = v[j];
                     group_sync(group);
-                    const float *from = buffer + r * kStagingRow + lane % 4 * 8;
+                    const float *from = buffer + r * kStagingRow + lane % 8 * 8;
                     if (c + r < t.rows) {
 #pragma unroll
-                        for (int i = 0; i < (P == kUp ? 2 : 4); ++i) {
-                            const int f = feature + i * 32 + lane % 4 * 8;
+                        for (int i = 0; i < (P == kUp ? 1 : 2); ++i) {
+                            const int f = feature + i * 64 + lane % 8 * 8;
                             [[maybe_unused]] float a[8], b[8], w[8];
-                            load8(from + i * 32, a);
+                            load8(from + i * 64, a);
                             if constexpr (P == kUp) {
                                 if (f >= m.inner) break;
-                                load8(from + 64 + i * 32, b);
+                                load8(from + 64, b);
                                 if (gu != nullptr) {
                                     store8(gu + row * 2 * m.inner + f, a);
                                     store8(gu + row * 2 * m.inner + m.inner + f, b);
