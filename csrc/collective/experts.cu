@@ -276,6 +276,12 @@ template <Product P> struct Tiles {
     }
 };
 
+// The first kernel of a call (kUp, kBack) waits for the kernels before the call.  The others may start
+// while their predecessor in the call runs, and load early what that one does not write.
+template <Product P> constexpr bool kFirstOfCall = P == kUp || P == kBack;
+template <Product P> constexpr bool kEarlyA = P == kDown || P == kInput || P == kGradOut;
+template <Product P> constexpr bool kEarlyB = P == kGradIn || P == kGradOut;
+
 template <Product P> __device__ __forceinline__ int steps_of(const Shape &m, const Tile &t) {
     if (kWeightGrad<P>) return ceil_div(t.rows, kDepth);
     if (P == kInput) return 2 * ceil_div(m.inner, kDepth);
@@ -291,7 +297,7 @@ __device__ void scan_counts(const Shape &m, Shared &sh, int *first) {
     for (int e = e0; e < e1; ++e) {
         const int c = m.counts[e];
         bad |= c < 0;
-        own += max(c, 0);
+        own += first[e] = max(c, 0);
     }
     long long upto = own;
     for (int o = 1; o < 32; o *= 2) {
@@ -303,8 +309,9 @@ __device__ void scan_counts(const Shape &m, Shared &sh, int *first) {
     for (int w = 0; w < warp; ++w) upto += sh.scan[w];
     long long at = upto - own;
     for (int e = e0; e < e1; ++e) {
+        const int c = first[e];
         first[e] = int(min(at, (long long)m.rows));
-        at += max(m.counts[e], 0);
+        at += c;
     }
     if (threadIdx.x == kThreads - 1) {
         first[m.nexp] = int(min(upto, (long long)m.rows));
@@ -367,7 +374,9 @@ template <Product P> struct Loader {
     const Shape &m;
     Shared &sh;
     const uint32_t stage0, full, tail, rank;
+    const int part_steps;        // kInput: steps through the gate's half of the depth
     uint32_t s = 0, parity = 1;  // the next stage, and the phase of its barrier that frees it
+    bool started = false;
 
     __device__ __forceinline__ bool load_tile(const Tile &t) {
         if constexpr (kWeightGrad<P>) {
@@ -384,59 +393,88 @@ template <Product P> struct Loader {
 
     // All steps of a tile, with LOAD of B's rows from this CTA's half on.
     template <int LOAD> __device__ __forceinline__ bool load_steps(const Tile &t, int half) {
-        const int steps = steps_of<P>(m, t), feature = t.feature + int(rank) * (kTileFeatures<P> / 2);
-        int row = t.first + (kWeightGrad<P> ? 0 : int(rank) * half);  // weight gradients: the step's first row
-        int depth = 0, part = 0;
-        for (int k = 0; k < steps; ++k) {
+        const int steps = steps_of<P>(m, t);
+        int k = 0;
+        if (!started) {
+            // The first steps: what does not come from the kernel before, then, once it is over, the rest.
+            const int filled = min(steps, kStages);
+            for (; k < filled; ++k) {
+                mbar_expect_cluster(barrier(t, k, k), kOperandBytes + uint32_t(LOAD) * kDepth * 2);
+                if (kEarlyA<P>) load_a(t, k, k);
+                if (kEarlyB<P>) load_b<LOAD>(t, half, k, k);
+            }
+            if (!kEarlyA<P> || !kEarlyB<P>) wait_previous();
+            for (k = 0; k < filled; ++k) {
+                if (!kEarlyA<P>) load_a(t, k, k);
+                if (!kEarlyB<P>) load_b<LOAD>(t, half, k, k);
+            }
+            started = true;
+            if ((s = uint32_t(filled)) == kStages) s = 0, parity ^= 1;
+        }
+        for (; k < steps; ++k) {
             if (!mbar_wait(smem_addr(&sh.empty[s]), parity, sh, m.status)) return false;
-            const uint32_t a = stage0 + s * 2 * kOperandBytes, b = a + kOperandBytes;
-            uint32_t bar = full + s * 8;
-            // A last step that reaches past the group goes to the warp that clears its tail.
-            if (kWeightGrad<P> && (k + 1) * kDepth > t.rows) bar = tail + s * 8;
-            mbar_expect_cluster(bar, kOperandBytes + uint32_t(LOAD) * kDepth * 2);
-            if constexpr (P == kUp) {
-                tma_load(a, &maps.a, bar, depth, feature, 0, t.expert);
-            } else if constexpr (P == kDown) {
-                tma_load(a, &maps.a, bar, depth, feature, t.expert);
-            } else {
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const uint32_t dst = a + uint32_t(c) * kOperandBytes / 2;
-                    const int f = feature + c * 64;
-                    if constexpr (P == kBack)
-                        tma_load(dst, &maps.a, bar, f, depth, t.expert);
-                    else if constexpr (P == kInput)
-                        tma_load(dst, &maps.a, bar, f, depth, part, t.expert);
-                    else if constexpr (P == kGradOut)
-                        tma_load(dst, &maps.a, bar, f, row);
-                    else
-                        tma_load(dst, &maps.a, bar, f, t.part, row);
-                }
-            }
-            if constexpr (kWeightGrad<P>) {
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    tma_load(b + uint32_t(c) * kOperandBytes / 2, &maps.b[0], bar, t.column + int(rank) * kHalf + c * 64,
-                             row);
-                row += kDepth;
-            } else {
-                int r = 0;
-#pragma unroll
-                for (int i = 0; i < kBoxes; ++i) {
-                    constexpr int kFirst = kHalf;
-                    if ((LOAD & kFirst >> i) == 0) continue;
-                    if constexpr (P == kInput)
-                        tma_load(b + uint32_t(r) * kDepth * 2, &maps.b[i], bar, depth, part, row + r);
-                    else
-                        tma_load(b + uint32_t(r) * kDepth * 2, &maps.b[i], bar, depth, row + r);
-                    r += kFirst >> i;
-                }
-            }
-            depth += kDepth;
-            if (P == kInput && depth >= m.inner && part == 0) depth = 0, part = 1;
+            mbar_expect_cluster(barrier(t, k, s), kOperandBytes + uint32_t(LOAD) * kDepth * 2);
+            load_a(t, k, s);
+            load_b<LOAD>(t, half, k, s);
             if (++s == kStages) s = 0, parity ^= 1;
         }
         return true;
+    }
+
+    // Where a step's bytes are counted.  A last step that reaches past the group goes to the warp that
+    // clears its tail.
+    __device__ __forceinline__ uint32_t barrier(const Tile &t, int k, uint32_t stage) const {
+        return (kWeightGrad<P> && (k + 1) * kDepth > t.rows ? tail : full) + stage * 8;
+    }
+
+    __device__ __forceinline__ void load_a(const Tile &t, int k, uint32_t stage) const {
+        const uint32_t a = stage0 + stage * 2 * kOperandBytes, bar = barrier(t, k, stage);
+        const int feature = t.feature + int(rank) * (kTileFeatures<P> / 2), depth = k * kDepth;
+        if constexpr (P == kUp) {
+            tma_load(a, &maps.a, bar, depth, feature, 0, t.expert);
+        } else if constexpr (P == kDown) {
+            tma_load(a, &maps.a, bar, depth, feature, t.expert);
+        } else {
+            const int part = P == kInput ? k >= part_steps : 0;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const uint32_t dst = a + uint32_t(c) * kOperandBytes / 2;
+                const int f = feature + c * 64;
+                if constexpr (P == kBack)
+                    tma_load(dst, &maps.a, bar, f, depth, t.expert);
+                else if constexpr (P == kInput)
+                    tma_load(dst, &maps.a, bar, f, depth - part * part_steps * kDepth, part, t.expert);
+                else if constexpr (P == kGradOut)
+                    tma_load(dst, &maps.a, bar, f, t.first + depth);
+                else
+                    tma_load(dst, &maps.a, bar, f, t.part, t.first + depth);
+            }
+        }
+    }
+
+    template <int LOAD> __device__ __forceinline__ void load_b(const Tile &t, int half, int k, uint32_t stage) const {
+        const uint32_t b = stage0 + stage * 2 * kOperandBytes + kOperandBytes, bar = barrier(t, k, stage);
+        const int depth = k * kDepth;
+        if constexpr (kWeightGrad<P>) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                tma_load(b + uint32_t(c) * kOperandBytes / 2, &maps.b[0], bar, t.column + int(rank) * kHalf + c * 64,
+                         t.first + depth);
+        } else {
+            const int row = t.first + int(rank) * half, part = P == kInput ? k >= part_steps : 0;
+            int r = 0;
+#pragma unroll
+            for (int i = 0; i < kBoxes; ++i) {
+                constexpr int kFirst = kHalf;
+                if ((LOAD & kFirst >> i) == 0) continue;
+                if constexpr (P == kInput)
+                    tma_load(b + uint32_t(r) * kDepth * 2, &maps.b[i], bar, depth - part * part_steps * kDepth, part,
+                             row + r);
+                else
+                    tma_load(b + uint32_t(r) * kDepth * 2, &maps.b[i], bar, depth, row + r);
+                r += kFirst >> i;
+            }
+        }
     }
 };
 
@@ -455,7 +493,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t stage0 = smem_addr(tiles_mem);
     constexpr bool kInnerA = kFeaturesInner<P>, kInnerB = kWeightGrad<P>;
 
-    launch_next();
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(smem_addr(&sh.full[s]), 2);   // both CTAs' loads, counted in the leading CTA
@@ -476,21 +513,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     if (threadIdx.x >= 32 && threadIdx.x < 32 + 1 + (kWeightGrad<P> ? 1 : kBoxes))
         asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a + (threadIdx.x - 32)) : "memory");
-    wait_previous();
-    scan_counts(m, sh, first);
     fence_before();
-    __syncthreads();
     cluster_sync();
     fence_after();
+    if (kFirstOfCall<P>) wait_previous();
+    launch_next();  // only now, so that the next kernel of the call finds the call's inputs complete
+    scan_counts(m, sh, first);
+    __syncthreads();
     const uint32_t tmem = sh.tmem;
 
     if (warp == 0 && lane == 0) {
         // Loads: this CTA's features and its half of the rows (or columns), stage after stage.
-        Loader<P> loader{maps, m, sh, stage0, map_to(smem_addr(sh.full), 0), map_to(smem_addr(sh.tail), rank), rank};
+        Loader<P> loader{maps, m, sh, stage0, map_to(smem_addr(sh.full), 0), map_to(smem_addr(sh.tail), rank), rank,
+                         ceil_div(m.inner, kDepth)};
         Tiles<P> tiles(m, first);
         Tile t;
         for (int at = pair; tiles.next(at, t); at += pairs)
             if (!loader.load_tile(t)) break;
+        wait_previous();  // in any case: a kernel is over only when those before it are
     } else if (warp == 1 && lane == 0 && rank == 0) {
         // Matrix instructions of the pair.
         constexpr uint32_t kType = std::is_same_v<T, __nv_bfloat16> ? 1 : 0;
