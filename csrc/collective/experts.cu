@@ -47,11 +47,13 @@ constexpr int kPairFeatures = 256;
 constexpr int kMaxN = 256;
 constexpr int kStepN = 32;
 constexpr int kDepth = 64;          // elements per stage along the summed dimension: 128 bytes
-constexpr int kBoxes = 4;            // TMA boxes of 128, 64, 32 and 16 rows
-constexpr int kStages = 6;
+constexpr int kBoxes = 4;           // TMA boxes of 128, 64, 32 and 16 rows
+constexpr int kMaxStages = 10;
+constexpr int kMaxSplit = 4;
 constexpr int kChunk = 16;          // rows (or columns of a gradient) that an epilogue group moves at once
 constexpr int kBand = 8;            // row tiles that run through all features before the next
-constexpr uint32_t kOperandBytes = kHalf * kDepth * 2;  // one CTA's half of A, or of B, in a stage
+constexpr uint32_t kOperandBytes = kHalf * kDepth * 2;  // one CTA's half of A, or of B for the largest N
+constexpr uint32_t kRingBytes = 6 * 2 * kOperandBytes;  // 6 stages for the largest N, 10 for the smallest
 constexpr int kStagingRow = kHalf + 4;                  // floats; the 4 keep 16-byte reads apart
 constexpr uint32_t kStagingBytes = kChunk * kStagingRow * 4;
 constexpr uint64_t kWaitNs = 5ull * 1000 * 1000 * 1000;
@@ -65,16 +67,19 @@ struct Shape {
     const int32_t *counts;
     unsigned int *status;
     int rows, nexp, hidden, inner, act;
+    int stages;            // of the ring, and the bytes of one: B's part is what the rows can need
+    uint32_t stage_bytes;
 };
 
 struct Shared {
-    alignas(8) uint64_t full[kStages], empty[kStages], tail[kStages], tmem_full[2], tmem_empty[2];
+    alignas(8) uint64_t full[kMaxStages], empty[kMaxStages], tail[kMaxStages], tmem_full[2], tmem_empty[2];
     uint32_t tmem;
     int aborted;
+    int row_tiles;  // of all experts, at most kMaxN rows each
     long long scan[kThreads / 32];
 };
 constexpr size_t shared_bytes(int nexp) {
-    return 1024 + kStages * 2 * kOperandBytes + 2 * kStagingBytes + sizeof(Shared) + (size_t(nexp) + 1) * 4;
+    return 1024 + kRingBytes + 2 * kStagingBytes + sizeof(Shared) + (size_t(nexp) + 1) * 4;
 }
 static_assert(shared_bytes(UGDR_X_EXPERTS_MAX) <= 232448, "227 KB of shared memory per CTA");
 
@@ -90,6 +95,14 @@ __device__ __forceinline__ uint32_t cta_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t n;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+    return n;
+}
+__device__ __forceinline__ void store_cluster(uint32_t addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 // The same shared address in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
@@ -162,10 +175,10 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, u
 // Operand descriptor for 128-byte swizzled tiles (rows of 128 bytes, atoms of 8 rows).  With the
 // summed dimension inner, 8 features to an atom and 1024 bytes to the next 8.  With the features
 // inner, 64 of them to an atom of 8 summed positions, 1024 bytes to the next 8 positions and one
-// tile of 64 x 128 bytes to the next 64 features.
+// tile of 64 x 128 bytes to the next 64 features.  (Above its 18 bits an address names the CTA.)
 template <bool FEATURES_INNER> __device__ __forceinline__ uint64_t operand(uint32_t addr) {
     const uint64_t leading = FEATURES_INNER ? kDepth * 128 / 16 : 1, stride = 1024 / 16;
-    return uint64_t(addr >> 4) | leading << 16 | stride << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+    return uint64_t(addr >> 4 & 0x3fff) | leading << 16 | stride << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
 }
 // From one instruction's 16 summed positions to the next's, in the descriptor's address field.
 template <bool FEATURES_INNER> constexpr uint64_t kOperandStep = FEATURES_INNER ? 16 * 128 / 16 : 16 * 2 / 16;
@@ -176,11 +189,12 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
                  "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
                  : "memory");
 }
-// Arrives on `bar` of both CTAs once the instructions issued before are done.
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
+// Arrives on `bar` of both CTAs of the pair that begins at cluster rank `leader`, once the
+// instructions issued before are done.
+__device__ __forceinline__ void mma_commit(uint32_t bar, uint32_t leader) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
                      bar),
-                 "h"(uint16_t(3))
+                 "h"(uint16_t(3u << leader))
                  : "memory");
 }
 // Programmatic launches: the next kernel of the stream may begin its set-up, and this one waits here
@@ -199,6 +213,14 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[kChunk]) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
                    "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
                    "=r"(r[15])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[8]) {
+    uint32_t *r = reinterpret_cast<uint32_t *>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(addr)
                  : "memory");
 }
@@ -226,35 +248,69 @@ struct Tile {
     int first;    // rows products: the tile's first row.  Weight gradients: the group's
     int rows;     // likewise, of the tile or the group
     int column;   // weight gradients: first of the N
+
+    // Rows that the tile's first accumulator takes; a wide tile's second one takes the others.
+    __device__ __forceinline__ int front() const {
+        return rows <= kMaxN ? rows : ceil_div(ceil_div(rows, 2), kStepN) * kStepN;
+    }
 };
 
 // Features of a tile of the pair: with kUp 128 of the gate and the same 128 of the up projection.
 template <Product P> constexpr int kTileFeatures = P == kUp ? kPairFeatures / 2 : kPairFeatures;
 
+template <Product P> __device__ __forceinline__ int steps_of(const Shape &m, int rows) {
+    if (kWeightGrad<P>) return ceil_div(rows, kDepth);
+    if (P == kInput) return 2 * ceil_div(m.inner, kDepth);
+    return ceil_div(P == kDown ? m.inner : m.hidden, kDepth);
+}
+
 // Walks the tile list in order: next() finds tile t for increasing t.
 template <Product P> struct Tiles {
     const int *first;  // first row of each expert's group, and the end of the last
-    int nexp, mtiles, mparts, ntiles;
-    int expert, base, size;
+    int nexp, mtiles, mparts, ntiles, steps;
+    bool wide;
+    int expert = -1, base = 0, size = 0, n = 0, columns = 0, per = 0;
 
-    __device__ Tiles(const Shape &m, const int *first_) : first(first_), nexp(m.nexp), expert(-1), base(0), size(0) {
+    // `workers`: pairs (or clusters) that share the list.
+    __device__ Tiles(const Shape &m, const int *first_, int row_tiles, int workers) : first(first_), nexp(m.nexp) {
         const int features = P == kUp || P == kBack || P == kGradIn ? m.inner : m.hidden;
         mparts = ceil_div(features, kTileFeatures<P>);
         mtiles = P == kGradIn ? 2 * mparts : mparts;
         ntiles = P == kGradOut ? ceil_div(m.inner, kMaxN) : P == kGradIn ? ceil_div(m.hidden, kMaxN) : 0;
+        steps = kWeightGrad<P> ? 0 : steps_of<P>(m, 0);
+        // Wide tiles leave work for fewer pairs: only where there is plenty.
+        wide = !kWeightGrad<P> && m.stage_bytes == 2 * kOperandBytes && int64_t(row_tiles) * mtiles >= 4 * workers;
+    }
+    // How the expert's rows are cut into tiles: of about the same size, all but the last a multiple
+    // of kStepN.  Clocks of a step: 2 per row for the products, and 64 bytes per clock for loading,
+    // which is 256 for the features and 1 per row.  So two tiles of 160 rows would wait for their
+    // loads, and one wide tile of 288, which loads the features once and fills the accumulators of
+    // two, is faster (32 experts of 300 rows, 7168 x 2048: 0.87 ms with tiles of at most 256 rows,
+    // 0.69 with wide ones), as long as its many steps outweigh that its accumulators, some 32 clocks
+    // per row, are moved out while no products run.
+    __device__ __forceinline__ void cut() {
+        columns = ceil_div(n, kMaxN);
+        per = columns == 0 ? 0 : ceil_div(ceil_div(n, columns), kStepN) * kStepN;
+        if (!wide || columns < 2) return;
+        const int wcolumns = ceil_div(n, 2 * kMaxN), wper = ceil_div(ceil_div(n, wcolumns), kStepN) * kStepN;
+        if (wper <= kMaxN) return;
+        const int64_t cost = int64_t(columns) * max(2 * per, 256 + per);
+        const int64_t wcost = int64_t(wcolumns) * (max(2 * wper, 256 + wper) + 32 * wper / steps);
+        if (wcost < cost) columns = wcolumns, per = wper;
     }
     __device__ __forceinline__ bool next(int t, Tile &out) {
-        int n = 0;
         while (t >= base + size) {
             if (++expert >= nexp) return false;
             base += size;
             n = first[expert + 1] - first[expert];
-            size = mtiles * (kWeightGrad<P> ? ntiles : ceil_div(n, kMaxN));
+            if (kWeightGrad<P>)
+                columns = ntiles;
+            else
+                cut();
+            size = mtiles * columns;
         }
-        n = first[expert + 1] - first[expert];
         // Bands of kBand N tiles; inside, all N tiles of one feature tile before the next, so that
         // pairs that run together share weights and rows in the L2.
-        const int columns = kWeightGrad<P> ? ntiles : ceil_div(n, kMaxN);
         const int local = t - base, band = local / (kBand * mtiles), in_band = local - band * kBand * mtiles;
         const int width = min(kBand, columns - band * kBand);
         const int mtile = in_band / width, ntile = band * kBand + in_band - mtile * width;
@@ -266,8 +322,6 @@ template <Product P> struct Tiles {
             out.rows = n;
             out.column = ntile * kMaxN;
         } else {
-            // Tiles of about the same size, none above kMaxN, all but the last a multiple of kStepN.
-            const int per = ceil_div(ceil_div(n, columns), kStepN) * kStepN;
             out.first = first[expert] + ntile * per;
             out.rows = min(per, n - ntile * per);
             out.column = 0;
@@ -281,12 +335,6 @@ template <Product P> struct Tiles {
 template <Product P> constexpr bool kFirstOfCall = P == kUp || P == kBack;
 template <Product P> constexpr bool kEarlyA = P == kDown || P == kInput || P == kGradOut;
 template <Product P> constexpr bool kEarlyB = P == kGradIn || P == kGradOut;
-
-template <Product P> __device__ __forceinline__ int steps_of(const Shape &m, const Tile &t) {
-    if (kWeightGrad<P>) return ceil_div(t.rows, kDepth);
-    if (P == kInput) return 2 * ceil_div(m.inner, kDepth);
-    return ceil_div(P == kDown ? m.inner : m.hidden, kDepth);
-}
 
 // First rows of the groups into first[0 .. nexp]: a scan over the block's threads.
 __device__ void scan_counts(const Shape &m, Shared &sh, int *first) {
@@ -308,11 +356,14 @@ __device__ void scan_counts(const Shape &m, Shared &sh, int *first) {
     __syncthreads();
     for (int w = 0; w < warp; ++w) upto += sh.scan[w];
     long long at = upto - own;
+    int row_tiles = 0;
     for (int e = e0; e < e1; ++e) {
         const int c = first[e];
         first[e] = int(min(at, (long long)m.rows));
         at += c;
+        row_tiles += ceil_div(int(min(at, (long long)m.rows)) - first[e], kMaxN);
     }
+    if (row_tiles > 0) atomicAdd(&sh.row_tiles, row_tiles);
     if (threadIdx.x == kThreads - 1) {
         first[m.nexp] = int(min(upto, (long long)m.rows));
         bad |= upto > m.rows;
@@ -343,6 +394,13 @@ __device__ __forceinline__ void load8(const float *p, float *v) {
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
+__device__ __forceinline__ void add8(const float *p, float (&v)[8]) {
+    float w[8];
+    load8(p, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += w[j];
+}
+
 // a(g) and a'(g).  The reciprocal is the approximate one (1 ulp): 1 + exp(-g) is between 1 and
 // infinity, whose reciprocal is the 0 that belongs there.
 struct Act {
@@ -366,6 +424,18 @@ struct Maps {
     CUtensorMap a, b[kBoxes];
 };
 
+// A place in the ring of stages: its shared addresses, kept rather than computed, because the two
+// threads that walk the ring are what short steps wait for.
+struct Ring {
+    uint32_t stage, bar;  // the stage, and an offset into each array of barriers
+    uint32_t parity;
+    __device__ __forceinline__ void next(const Shape &m, uint32_t stage0) {
+        stage += m.stage_bytes;
+        bar += 8;
+        if (bar == uint32_t(m.stages) * 8) stage = stage0, bar = 0, parity ^= 1;
+    }
+};
+
 // The thread that issues a CTA's loads.  Its loop is what a stage of few rows takes longest for, so
 // it is kept short: a loop of its own for every set of boxes, whose maps are then known.  (Picking
 // the map by an index made single rows per expert take 1.3 times as long.)
@@ -373,72 +443,100 @@ template <Product P> struct Loader {
     const Maps &maps;
     const Shape &m;
     Shared &sh;
-    const uint32_t stage0, full, tail, rank;
-    const int part_steps;        // kInput: steps through the gate's half of the depth
-    uint32_t s = 0, parity = 1;  // the next stage, and the phase of its barrier that frees it
+    const uint32_t stage0, empty, full, tail, rank;  // barriers: `full` in the leading CTA
+    const int part_steps;                            // kInput: steps through the gate's half of the depth
+    Ring at;
     bool started = false;
 
-    __device__ __forceinline__ bool load_tile(const Tile &t) {
+    __device__ __forceinline__ bool wait() { return mbar_wait(empty + at.bar, at.parity, sh, m.status); }
+
+    // Steps [k0, k1) of a tile.
+    __device__ __forceinline__ bool load_tile(const Tile &t, int k0, int k1) {
         if constexpr (kWeightGrad<P>) {
-            return load_steps<kHalf>(t, kHalf);
+            return load_steps<kHalf>(t, kHalf, k0, k1);
         } else {
-            const int half = ceil_div(t.rows, kStepN) * kStepN / 2;
-            return half > 96   ? load_steps<128>(t, half)
-                   : half > 64 ? load_steps<96>(t, half)
-                   : half > 32 ? load_steps<64>(t, half)
-                   : half > 16 ? load_steps<32>(t, half)
-                               : load_steps<16>(t, half);
+            const int half = ceil_div(t.front(), kStepN) * kStepN / 2;
+            if (t.rows > kMaxN) return half > 96 ? load_wide<128>(t, half, k1) : load_wide<96>(t, half, k1);
+            return half > 96   ? load_steps<128>(t, half, k0, k1)
+                   : half > 64 ? load_steps<96>(t, half, k0, k1)
+                   : half > 32 ? load_steps<64>(t, half, k0, k1)
+                   : half > 16 ? load_steps<32>(t, half, k0, k1)
+                               : load_steps<16>(t, half, k0, k1);
         }
     }
 
-    // All steps of a tile, with LOAD of B's rows from this CTA's half on.
-    template <int LOAD> __device__ __forceinline__ bool load_steps(const Tile &t, int half) {
-        const int steps = steps_of<P>(m, t);
-        int k = 0;
+    // With LOAD of B's rows from this CTA's half on.
+    template <int LOAD> __device__ __forceinline__ bool load_steps(const Tile &t, int half, int k0, int k1) {
+        constexpr uint32_t kBytes = kOperandBytes + uint32_t(LOAD) * kDepth * 2;
+        int k = k0;
         if (!started) {
             // The first steps: what does not come from the kernel before, then, once it is over, the rest.
-            const int filled = min(steps, kStages);
-            for (; k < filled; ++k) {
-                mbar_expect_cluster(barrier(t, k, k), kOperandBytes + uint32_t(LOAD) * kDepth * 2);
-                if (kEarlyA<P>) load_a(t, k, k);
-                if (kEarlyB<P>) load_b<LOAD>(t, half, k, k);
+            const int filled = min(k1, k0 + m.stages);
+            const Ring begin = at;
+            for (; k < filled; ++k, at.next(m, stage0)) {
+                const uint32_t bar = barrier(t, k);
+                mbar_expect_cluster(bar, kBytes);
+                if (kEarlyA<P>) load_a(t, k, bar);
+                if (kEarlyB<P>) load_b<LOAD>(t, t.first, half, k, bar);
             }
-            if (!kEarlyA<P> || !kEarlyB<P>) wait_previous();
-            for (k = 0; k < filled; ++k) {
-                if (!kEarlyA<P>) load_a(t, k, k);
-                if (!kEarlyB<P>) load_b<LOAD>(t, half, k, k);
+            if (!kEarlyA<P> || !kEarlyB<P>) {
+                wait_previous();
+                at = begin;
+                for (k = k0; k < filled; ++k, at.next(m, stage0)) {
+                    const uint32_t bar = barrier(t, k);
+                    if (!kEarlyA<P>) load_a(t, k, bar);
+                    if (!kEarlyB<P>) load_b<LOAD>(t, t.first, half, k, bar);
+                }
             }
             started = true;
-            if ((s = uint32_t(filled)) == kStages) s = 0, parity ^= 1;
         }
-        for (; k < steps; ++k) {
-            if (!mbar_wait(smem_addr(&sh.empty[s]), parity, sh, m.status)) return false;
-            mbar_expect_cluster(barrier(t, k, s), kOperandBytes + uint32_t(LOAD) * kDepth * 2);
-            load_a(t, k, s);
-            load_b<LOAD>(t, half, k, s);
-            if (++s == kStages) s = 0, parity ^= 1;
+        for (; k < k1; ++k, at.next(m, stage0)) {
+            if (!wait()) return false;
+            const uint32_t bar = barrier(t, k);
+            mbar_expect_cluster(bar, kBytes);
+            load_a(t, k, bar);
+            load_b<LOAD>(t, t.first, half, k, bar);
+        }
+        return true;
+    }
+
+    // A wide tile: a stage with the features and the first accumulator's rows, then one with the
+    // second's rows.
+    template <int LOAD> __device__ __forceinline__ bool load_wide(const Tile &t, int half, int steps) {
+        if (!started) wait_previous();
+        started = true;
+        const int front = t.front(), half2 = ceil_div(t.rows - front, kStepN) * kStepN / 2;
+        for (int k = 0; k < steps; ++k) {
+            if (!wait()) return false;
+            mbar_expect_cluster(full + at.bar, kOperandBytes + uint32_t(LOAD) * kDepth * 2);
+            load_a(t, k, full + at.bar);
+            load_b<LOAD>(t, t.first, half, k, full + at.bar);
+            at.next(m, stage0);
+            if (!wait()) return false;
+            mbar_expect_cluster(full + at.bar, uint32_t(LOAD) * kDepth * 2);
+            load_b<LOAD>(t, t.first + front, half2, k, full + at.bar);
+            at.next(m, stage0);
         }
         return true;
     }
 
     // Where a step's bytes are counted.  A last step that reaches past the group goes to the warp that
     // clears its tail.
-    __device__ __forceinline__ uint32_t barrier(const Tile &t, int k, uint32_t stage) const {
-        return (kWeightGrad<P> && (k + 1) * kDepth > t.rows ? tail : full) + stage * 8;
+    __device__ __forceinline__ uint32_t barrier(const Tile &t, int k) const {
+        return (kWeightGrad<P> && (k + 1) * kDepth > t.rows ? tail : full) + at.bar;
     }
 
-    __device__ __forceinline__ void load_a(const Tile &t, int k, uint32_t stage) const {
-        const uint32_t a = stage0 + stage * 2 * kOperandBytes, bar = barrier(t, k, stage);
+    __device__ __forceinline__ void load_a(const Tile &t, int k, uint32_t bar) const {
         const int feature = t.feature + int(rank) * (kTileFeatures<P> / 2), depth = k * kDepth;
         if constexpr (P == kUp) {
-            tma_load(a, &maps.a, bar, depth, feature, 0, t.expert);
+            tma_load(at.stage, &maps.a, bar, depth, feature, 0, t.expert);
         } else if constexpr (P == kDown) {
-            tma_load(a, &maps.a, bar, depth, feature, t.expert);
+            tma_load(at.stage, &maps.a, bar, depth, feature, t.expert);
         } else {
             const int part = P == kInput ? k >= part_steps : 0;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const uint32_t dst = a + uint32_t(c) * kOperandBytes / 2;
+                const uint32_t dst = at.stage + uint32_t(c) * kOperandBytes / 2;
                 const int f = feature + c * 64;
                 if constexpr (P == kBack)
                     tma_load(dst, &maps.a, bar, f, depth, t.expert);
@@ -452,8 +550,9 @@ template <Product P> struct Loader {
         }
     }
 
-    template <int LOAD> __device__ __forceinline__ void load_b(const Tile &t, int half, int k, uint32_t stage) const {
-        const uint32_t b = stage0 + stage * 2 * kOperandBytes + kOperandBytes, bar = barrier(t, k, stage);
+    template <int LOAD>
+    __device__ __forceinline__ void load_b(const Tile &t, int first, int half, int k, uint32_t bar) const {
+        const uint32_t b = at.stage + kOperandBytes;
         const int depth = k * kDepth;
         if constexpr (kWeightGrad<P>) {
 #pragma unroll
@@ -461,7 +560,7 @@ template <Product P> struct Loader {
                 tma_load(b + uint32_t(c) * kOperandBytes / 2, &maps.b[0], bar, t.column + int(rank) * kHalf + c * 64,
                          t.first + depth);
         } else {
-            const int row = t.first + int(rank) * half, part = P == kInput ? k >= part_steps : 0;
+            const int row = first + int(rank) * half, part = P == kInput ? k >= part_steps : 0;
             int r = 0;
 #pragma unroll
             for (int i = 0; i < kBoxes; ++i) {
@@ -478,24 +577,128 @@ template <Product P> struct Loader {
     }
 };
 
+// The thread that issues a pair's matrix instructions.
+template <typename T, Product P> struct Issuer {
+    const Shape &m;
+    Shared &sh;
+    const uint32_t stage0, full, empty, leader;
+    Ring at;
+
+    __device__ __forceinline__ bool wait() {
+        if (!mbar_wait(full + at.bar, at.parity, sh, m.status)) return false;
+        fence_after();
+        return true;
+    }
+    // One stage's products: A at `sa`, B at `sb`, `parts` times 16 deep.
+    __device__ __forceinline__ void multiply(uint32_t d, uint32_t sa, uint32_t sb, uint32_t idesc, int parts,
+                                             bool add) const {
+        constexpr bool kInnerA = kFeaturesInner<P>, kInnerB = kWeightGrad<P>;
+        const uint64_t a = operand<kInnerA>(sa), b = operand<kInnerB>(sb);
+        for (int i = 0; i < parts; ++i)
+            mma(d, a + i * kOperandStep<kInnerA>, b + i * kOperandStep<kInnerB>, idesc, add || i > 0);
+    }
+    // The instruction: its types, layouts and N.
+    static __device__ __forceinline__ uint32_t instruction(int rows) {
+        constexpr uint32_t kType = std::is_same_v<T, __nv_bfloat16> ? 1 : 0;
+        return 1u << 4 | kType << 7 | kType << 10 | uint32_t(kFeaturesInner<P>) << 15 | uint32_t(kWeightGrad<P>) << 16 |
+               uint32_t(kPairFeatures / 16) << 24 | uint32_t(ceil_div(rows, kStepN) * (kStepN / 8)) << 17;
+    }
+
+    // Steps [k0, k1) of a tile into the accumulator at d.
+    __device__ __forceinline__ bool run(const Tile &t, uint32_t d, int k0, int k1) {
+        const uint32_t idesc = instruction(kWeightGrad<P> ? kMaxN : t.rows);
+        for (int k = k0; k < k1; ++k, at.next(m, stage0)) {
+            if (!wait()) return false;
+            int parts = kDepth / 16;
+            if (kWeightGrad<P>) parts = min(parts, ceil_div(t.rows - k * kDepth, 16));
+            multiply(d, at.stage, at.stage + kOperandBytes, idesc, parts, k > k0);
+            mma_commit(empty + at.bar, leader);
+        }
+        return true;
+    }
+    // A wide tile into the accumulators at d and d2.
+    __device__ __forceinline__ bool run_wide(const Tile &t, uint32_t d, uint32_t d2, int steps) {
+        const uint32_t idesc = instruction(t.front()), idesc2 = instruction(t.rows - t.front());
+        for (int k = 0; k < steps; ++k, at.next(m, stage0)) {
+            if (!wait()) return false;
+            const uint32_t sa = at.stage, freed = empty + at.bar;
+            multiply(d, sa, sa + kOperandBytes, idesc, kDepth / 16, k > 0);
+            at.next(m, stage0);
+            if (!wait()) return false;
+            multiply(d2, sa, at.stage + kOperandBytes, idesc2, kDepth / 16, k > 0);
+            mma_commit(freed, leader);
+            mma_commit(empty + at.bar, leader);
+        }
+        return true;
+    }
+};
+
+// What a row product does with 8 of a row's features: `a` are their sums (kUp: the gate's, and `b`
+// the up projection's), `g` and `u` with kBack the projections that the forward pass kept.
 template <typename T, Product P>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    expert_kernel(const __grid_constant__ Maps maps, const Shape m, T *out, float *gu) {
+__device__ __forceinline__ void finish(const Shape &m, T *out, float *gu, int64_t row, int f, const float (&a)[8],
+                                       const float (&b)[8], const float (&g)[8], const float (&u)[8]) {
+    if constexpr (P == kUp) {
+        if (gu != nullptr) {
+            store8(gu + row * 2 * m.inner + f, a);
+            store8(gu + row * 2 * m.inner + m.inner + f, b);
+        }
+        float h[8];
+        if (m.act == UGDR_X_ACT_SILU) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] = silu(a[j]).a * b[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] = gelu(a[j]).a * b[j];
+        }
+        store8(out + row * m.inner + f, h);
+    } else if constexpr (P == kBack) {
+        float dg[8], du[8];
+        if (m.act == UGDR_X_ACT_SILU) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const Act s = silu(g[j]);
+                dg[j] = a[j] * u[j] * s.da;
+                du[j] = a[j] * s.a;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const Act s = gelu(g[j]);
+                dg[j] = a[j] * u[j] * s.da;
+                du[j] = a[j] * s.a;
+            }
+        }
+        store8(out + row * 2 * m.inner + f, dg);
+        store8(out + row * 2 * m.inner + m.inner + f, du);
+    } else {
+        store8(out + row * m.hidden + f, a);
+    }
+}
+
+// A kernel's shared memory, barriers, TMEM and row counts, set up by all threads of a cluster.
+struct Setup {
+    uint8_t *ring;
+    float *staging;
+    Shared *sh;
+    int *first;
+    uint32_t stage0, rank, leader;  // rank: 0 or 1 in the pair, whose first CTA is `leader` of the cluster
+};
+
+template <Product P> __device__ __forceinline__ Setup set_up(const Maps &maps, const Shape &m) {
     extern __shared__ uint8_t raw[];
-    uint8_t *tiles_mem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);
-    float *staging = reinterpret_cast<float *>(tiles_mem + kStages * 2 * kOperandBytes);
-    Shared &sh = *reinterpret_cast<Shared *>(reinterpret_cast<uint8_t *>(staging) + 2 * kStagingBytes);
-    int *first = reinterpret_cast<int *>(&sh + 1);
-
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t rank = cta_rank();
-    const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
-    const uint32_t stage0 = smem_addr(tiles_mem);
-    constexpr bool kInnerA = kFeaturesInner<P>, kInnerB = kWeightGrad<P>;
-
+    Setup k;
+    k.ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);
+    k.staging = reinterpret_cast<float *>(k.ring + kRingBytes);
+    k.sh = reinterpret_cast<Shared *>(reinterpret_cast<uint8_t *>(k.staging) + 2 * kStagingBytes);
+    k.first = reinterpret_cast<int *>(k.sh + 1);
+    k.stage0 = smem_addr(k.ring);
+    k.rank = cta_rank() & 1;
+    k.leader = cta_rank() - k.rank;
+    Shared &sh = *k.sh;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
-            mbar_init(smem_addr(&sh.full[s]), 2);   // both CTAs' loads, counted in the leading CTA
+        for (int s = 0; s < kMaxStages; ++s) {
+            mbar_init(smem_addr(&sh.full[s]), 2);  // both CTAs' loads, counted in the leading CTA
             mbar_init(smem_addr(&sh.empty[s]), 1);
             mbar_init(smem_addr(&sh.tail[s]), 1);
         }
@@ -503,10 +706,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             mbar_init(smem_addr(&sh.tmem_full[s]), 1);
             mbar_init(smem_addr(&sh.tmem_empty[s]), 16);  // 8 epilogue warps of each CTA
         }
-        sh.aborted = 0;
+        sh.aborted = sh.row_tiles = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 2) {
+    if (threadIdx.x / 32 == 2) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sh.tmem))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -518,67 +721,86 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fence_after();
     if (kFirstOfCall<P>) wait_previous();
     launch_next();  // only now, so that the next kernel of the call finds the call's inputs complete
-    scan_counts(m, sh, first);
+    scan_counts(m, sh, k.first);
     __syncthreads();
-    const uint32_t tmem = sh.tmem;
+    return k;
+}
+
+// The end of a kernel, for all threads of a cluster.
+__device__ __forceinline__ void tear_down(const Setup &k) {
+    __syncthreads();
+    if (k.sh->aborted) {  // loads and instructions that are still under way end within this time
+        for (const uint64_t since = gtime(); gtime() - since < 2'000'000;) __nanosleep(1000);
+    }
+    fence_before();
+    cluster_sync();
+    if (threadIdx.x / 32 == 2) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(k.sh->tmem) : "memory");
+    }
+}
+
+template <Product P> __device__ __forceinline__ Loader<P> loader_of(const Maps &maps, const Shape &m, const Setup &k) {
+    Shared &sh = *k.sh;
+    return {maps,
+            m,
+            sh,
+            k.stage0,
+            smem_addr(sh.empty),
+            map_to(smem_addr(sh.full), k.leader),
+            map_to(smem_addr(sh.tail), k.leader + k.rank),
+            k.rank,
+            ceil_div(m.inner, kDepth),
+            {k.stage0, 0, 1}};  // parity 1: every stage is free
+}
+template <typename T, Product P> __device__ __forceinline__ Issuer<T, P> issuer_of(const Shape &m, const Setup &k) {
+    return {m, *k.sh, k.stage0, smem_addr(k.sh->full), smem_addr(k.sh->empty), k.leader, {k.stage0, 0, 0}};
+}
+
+// One product, a pair of CTAs per tile.
+template <typename T, Product P>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    expert_kernel(const __grid_constant__ Maps maps, const Shape m, T *out, float *gu) {
+    const Setup k = set_up<P>(maps, m);
+    Shared &sh = *k.sh;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+    Tiles<P> tiles(m, k.first, sh.row_tiles, pairs);
+    Tile t;
+    uint32_t acc = 0;  // accumulators used so far: they take turns
 
     if (warp == 0 && lane == 0) {
-        // Loads: this CTA's features and its half of the rows (or columns), stage after stage.
-        Loader<P> loader{maps, m, sh, stage0, map_to(smem_addr(sh.full), 0), map_to(smem_addr(sh.tail), rank), rank,
-                         ceil_div(m.inner, kDepth)};
-        Tiles<P> tiles(m, first);
-        Tile t;
+        Loader<P> loader = loader_of<P>(maps, m, k);
         for (int at = pair; tiles.next(at, t); at += pairs)
-            if (!loader.load_tile(t)) break;
+            if (!loader.load_tile(t, 0, steps_of<P>(m, t.rows))) break;
         wait_previous();  // in any case: a kernel is over only when those before it are
-    } else if (warp == 1 && lane == 0 && rank == 0) {
-        // Matrix instructions of the pair.
-        constexpr uint32_t kType = std::is_same_v<T, __nv_bfloat16> ? 1 : 0;
-        constexpr uint32_t kBase = 1u << 4 | kType << 7 | kType << 10 | uint32_t(kInnerA) << 15 |
-                                   uint32_t(kInnerB) << 16 | uint32_t(kPairFeatures / 16) << 24;
-        Tiles<P> tiles(m, first);
-        Tile t;
-        uint32_t it = 0, acc = 0;
-        bool go = true;
-        for (int at = pair; go && tiles.next(at, t); at += pairs) {
-            const int steps = steps_of<P>(m, t);
-            if (steps == 0) continue;
-            const int n = kWeightGrad<P> ? kMaxN : ceil_div(t.rows, kStepN) * kStepN;
-            const uint32_t idesc = kBase | uint32_t(n / 8) << 17;
-            const uint32_t d = tmem + (acc & 1) * kMaxN;
-            if (!mbar_wait(smem_addr(&sh.tmem_empty[acc & 1]), (acc / 2 + 1) & 1, sh, m.status)) break;
+    } else if (warp == 1 && lane == 0 && k.rank == 0) {
+        Issuer<T, P> issuer = issuer_of<T, P>(m, k);
+        auto wait_accumulator = [&](uint32_t a) {
+            if (!mbar_wait(smem_addr(&sh.tmem_empty[a & 1]), (a / 2 + 1) & 1, sh, m.status)) return false;
             fence_after();
-            for (int k = 0; k < steps; ++k, ++it) {
-                const uint32_t s = it % kStages;
-                if (!mbar_wait(smem_addr(&sh.full[s]), (it / kStages) & 1, sh, m.status)) {
-                    go = false;
-                    break;
-                }
-                fence_after();
-                const uint32_t addr = stage0 + s * 2 * kOperandBytes;
-                const uint64_t a = operand<kInnerA>(addr), b = operand<kInnerB>(addr + kOperandBytes);
-                int parts = kDepth / 16;
-                if (kWeightGrad<P>) parts = min(parts, ceil_div(t.rows - k * kDepth, 16));
-                for (int i = 0; i < parts; ++i)
-                    mma(d, a + i * kOperandStep<kInnerA>, b + i * kOperandStep<kInnerB>, idesc, k + i > 0);
-                mma_commit(smem_addr(&sh.empty[s]));
-            }
-            if (go) mma_commit(smem_addr(&sh.tmem_full[acc & 1]));
-            ++acc;
+            return true;
+        };
+        for (int at = pair; tiles.next(at, t); at += pairs) {
+            const int steps = steps_of<P>(m, t.rows);
+            if (steps == 0) continue;
+            const uint32_t d = sh.tmem + (acc & 1) * kMaxN, d2 = sh.tmem + (~acc & 1) * kMaxN;
+            const bool wide = !kWeightGrad<P> && t.rows > kMaxN;
+            if (!wait_accumulator(acc) || (wide && !wait_accumulator(acc + 1))) break;
+            if (!(wide ? issuer.run_wide(t, d, d2, steps) : issuer.run(t, d, 0, steps))) break;
+            mma_commit(smem_addr(&sh.tmem_full[acc++ & 1]), k.leader);
+            if (wide) mma_commit(smem_addr(&sh.tmem_full[acc++ & 1]), k.leader);
         }
     } else if (warp == 2 && kWeightGrad<P>) {
         // Tails: the rows behind the group in its last step, up to the next 16, become zeros.
-        Tiles<P> tiles(m, first);
-        Tile t;
         uint32_t it = 0, phases = 0;
         for (int at = pair; tiles.next(at, t); at += pairs) {
-            const int steps = steps_of<P>(m, t), last = t.rows % kDepth;
-            it += uint32_t(steps);
+            const int last = t.rows % kDepth;
+            it += uint32_t(steps_of<P>(m, t.rows));
             if (last == 0) continue;
-            const uint32_t s = (it - 1) % kStages;
+            const uint32_t s = (it - 1) % uint32_t(m.stages);
             if (!mbar_wait(smem_addr(&sh.tail[s]), phases >> s & 1, sh, m.status)) break;
             phases ^= 1u << s;
-            uint8_t *stage = tiles_mem + s * 2 * kOperandBytes;
+            uint8_t *stage = k.ring + s * m.stage_bytes;
             const int clear = ceil_div(last, 16) * 16 - last;  // rows of 128 bytes, in each of 4 tiles
             for (int i = lane; i < clear * 4 * 8; i += 32) {
                 const int tile = i / (clear * 8), piece = i % (clear * 8);
@@ -586,136 +808,169 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(map_to(smem_addr(&sh.full[s]), 0));
+            if (lane == 0) mbar_arrive_cluster(map_to(smem_addr(&sh.full[s]), k.leader));
             __syncwarp();
         }
     } else if (warp >= 4) {
         // Finished accumulators.  This warp's TMEM lanes are features 32 (warp % 4) ... + 31; its
         // group of four warps takes every other chunk of columns.
         const int quarter = warp % 4, group = warp / 4 - 1;
-        const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
-        Tiles<P> tiles(m, first);
-        Tile t;
-        uint32_t acc = 0;
-        for (int at = pair; tiles.next(at, t); at += pairs) {
-            const bool none = steps_of<P>(m, t) == 0;
-            if (!none) {
-                if (!group_all(group, mbar_wait(smem_addr(&sh.tmem_full[acc & 1]), (acc / 2) & 1, sh, m.status)))
-                    break;
-                fence_after();
-            }
-            const uint32_t columns = lanes + (acc & 1) * kMaxN;
-            const int feature = t.feature + int(rank) * (kTileFeatures<P> / 2);
-            if constexpr (kWeightGrad<P>) {
-                // A thread has one row of the gradient and writes its columns.
-                const int width = P == kGradOut ? m.inner : m.hidden, height = P == kGradOut ? m.hidden : m.inner;
-                const int f = feature + quarter * 32 + lane;
-                T *row = out + ((int64_t(t.expert) * (P == kGradIn ? 2 : 1) + t.part) * height + f) * width + t.column;
-                for (int c = group * kChunk; c < kMaxN; c += 2 * kChunk) {
-                    float v[kChunk];
-                    if (none) {
-#pragma unroll
-                        for (int j = 0; j < kChunk; ++j) v[j] = 0.f;
-                    } else {
-                        tmem_load(columns + c, v);
-                    }
-                    if (f < height) {
-#pragma unroll
-                        for (int j = 0; j < kChunk; j += 8)
-                            if (t.column + c + j < width) store8(row + c + j, v + j);
-                    }
+        const uint32_t lanes = sh.tmem + (uint32_t(quarter * 32) << 16), empty = map_to(smem_addr(sh.tmem_empty), k.leader);
+        bool go = true;
+        for (int at = pair; go && tiles.next(at, t); at += pairs) {
+            const bool none = steps_of<P>(m, t.rows) == 0;
+            const int feature = t.feature + int(k.rank) * (kTileFeatures<P> / 2);
+            const int front = kWeightGrad<P> ? t.rows : t.front();
+            int from = 0;
+            do {  // once, or for both accumulators of a wide tile
+                if (!none) {
+                    const bool full = mbar_wait(smem_addr(&sh.tmem_full[acc & 1]), (acc / 2) & 1, sh, m.status);
+                    if (!(go = group_all(group, full))) break;
+                    fence_after();
                 }
-            } else {
-                // A chunk of rows at a time, turned around in shared memory: then 8 lanes hold 64 of a
-                // row's features, 8 next to each other per lane.
-                const int r = quarter * 4 + lane / 8;
-                for (int c = group * kChunk; c < t.rows; c += 2 * kChunk) {
-                    const int64_t row = t.first + c + r;
-                    [[maybe_unused]] float g[2][8], u[2][8];
-                    if constexpr (P == kBack) {  // under way while the accumulators are turned around
+                const uint32_t columns = lanes + (acc & 1) * kMaxN;
+                if constexpr (kWeightGrad<P>) {
+                    // A thread has one row of the gradient and writes its columns.
+                    const int width = P == kGradOut ? m.inner : m.hidden, height = P == kGradOut ? m.hidden : m.inner;
+                    const int f = feature + quarter * 32 + lane;
+                    T *row = out + ((int64_t(t.expert) * (P == kGradIn ? 2 : 1) + t.part) * height + f) * width + t.column;
+                    for (int c = group * kChunk; c < kMaxN; c += 2 * kChunk) {
+                        float v[kChunk];
+                        if (none) {
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const int f = feature + i * 64 + lane % 8 * 8;
-                            if (c + r < t.rows && f < m.inner) {
-                                load8(gu + row * 2 * m.inner + f, g[i]);
-                                load8(gu + row * 2 * m.inner + m.inner + f, u[i]);
-                            }
+                            for (int j = 0; j < kChunk; ++j) v[j] = 0.f;
+                        } else {
+                            tmem_load(columns + c, v);
+                        }
+                        if (f < height) {
+#pragma unroll
+                            for (int j = 0; j < kChunk; j += 8)
+                                if (t.column + c + j < width) store8(row + c + j, v + j);
                         }
                     }
-                    float v[kChunk];
-                    tmem_load(columns + c, v);
-                    float *buffer = staging + group * (kStagingBytes / 4);
+                } else {
+                    // A chunk of rows at a time, turned around in shared memory: then 8 lanes hold 64
+                    // of a row's features, 8 next to each other per lane.
+                    const int rows = from == 0 ? front : t.rows - front, r = quarter * 4 + lane / 8;
+                    float *buffer = k.staging + group * (kStagingBytes / 4);
+                    for (int c = group * kChunk; c < rows; c += 2 * kChunk) {
+                        const int64_t row = t.first + from + c + r;
+                        float g[2][8], u[2][8];
+                        if constexpr (P == kBack) {  // under way while the accumulators are turned around
 #pragma unroll
-                    for (int j = 0; j < kChunk; ++j) buffer[j * kStagingRow + quarter * 32 + lane] = v[j];
-                    group_sync(group);
-                    const float *from = buffer + r * kStagingRow + lane % 8 * 8;
-                    if (c + r < t.rows) {
+                            for (int i = 0; i < 2; ++i) {
+                                const int f = feature + i * 64 + lane % 8 * 8;
+                                if (c + r < rows && f < m.inner) {
+                                    load8(gu + row * 2 * m.inner + f, g[i]);
+                                    load8(gu + row * 2 * m.inner + m.inner + f, u[i]);
+                                }
+                            }
+                        }
+                        float v[kChunk];
+                        tmem_load(columns + c, v);
+#pragma unroll
+                        for (int j = 0; j < kChunk; ++j) buffer[j * kStagingRow + quarter * 32 + lane] = v[j];
+                        group_sync(group);
+                        const float *sums = buffer + r * kStagingRow + lane % 8 * 8;
 #pragma unroll
                         for (int i = 0; i < (P == kUp ? 1 : 2); ++i) {
                             const int f = feature + i * 64 + lane % 8 * 8;
-                            [[maybe_unused]] float a[8], b[8], w[8];
-                            load8(from + i * 64, a);
-                            if constexpr (P == kUp) {
-                                if (f >= m.inner) break;
-                                load8(from + 64, b);
-                                if (gu != nullptr) {
-                                    store8(gu + row * 2 * m.inner + f, a);
-                                    store8(gu + row * 2 * m.inner + m.inner + f, b);
-                                }
-                                if (m.act == UGDR_X_ACT_SILU) {
-#pragma unroll
-                                    for (int j = 0; j < 8; ++j) w[j] = silu(a[j]).a * b[j];
-                                } else {
-#pragma unroll
-                                    for (int j = 0; j < 8; ++j) w[j] = gelu(a[j]).a * b[j];
-                                }
-                                store8(out + row * m.inner + f, w);
-                            } else if constexpr (P == kBack) {
-                                if (f >= m.inner) break;
-                                if (m.act == UGDR_X_ACT_SILU) {
-#pragma unroll
-                                    for (int j = 0; j < 8; ++j) {
-                                        const Act s = silu(g[i][j]);
-                                        w[j] = a[j] * u[i][j] * s.da;
-                                        b[j] = a[j] * s.a;
-                                    }
-                                } else {
-#pragma unroll
-                                    for (int j = 0; j < 8; ++j) {
-                                        const Act s = gelu(g[i][j]);
-                                        w[j] = a[j] * u[i][j] * s.da;
-                                        b[j] = a[j] * s.a;
-                                    }
-                                }
-                                store8(out + row * 2 * m.inner + f, w);
-                                store8(out + row * 2 * m.inner + m.inner + f, b);
-                            } else {
-                                if (f >= m.hidden) break;
-                                store8(out + row * m.hidden + f, a);
-                            }
+                            if (c + r >= rows || f >= (P == kUp || P == kBack ? m.inner : m.hidden)) continue;
+                            float a[8], b[8];
+                            load8(sums + i * 64, a);
+                            if (P == kUp) load8(sums + 64, b);
+                            finish<T, P>(m, out, gu, row, f, a, b, g[i], u[i]);
                         }
+                        group_sync(group);  // the buffer is free again
                     }
-                    group_sync(group);  // the buffer is free again
                 }
-            }
-            if (!none) {
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(map_to(smem_addr(&sh.tmem_empty[acc & 1]), 0));
-                ++acc;
-            }
+                if (!none) {
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(empty + (acc & 1) * 8);
+                    ++acc;
+                }
+                from += front;
+            } while (!kWeightGrad<P> && from < t.rows);
         }
     }
-    __syncthreads();
-    if (sh.aborted) {  // loads and instructions that are still under way end within this time
-        for (const uint64_t since = gtime(); gtime() - since < 2'000'000;) __nanosleep(1000);
-    }
-    fence_before();
-    cluster_sync();
-    if (warp == 2) {
+    tear_down(k);
+}
+
+// One product of few tiles: the pairs of a cluster share a tile, each with a part of the steps, and
+// add their sums up through distributed shared memory, in the pairs' order.  A tile's K loop runs at
+// the latency of its ring, so one pair reads weights at a few hundred GB/s however idle the GPU is:
+// a [1, 5632] x [5632, 2048] product has 8 tiles, and took 26 us with a pair each.
+template <typename T, Product P>
+__global__ void __launch_bounds__(kThreads, 1)
+    expert_split_kernel(const __grid_constant__ Maps maps, const Shape m, T *out, float *gu) {
+    const Setup k = set_up<P>(maps, m);
+    Shared &sh = *k.sh;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int split = int(cluster_size()) / 2, part = int(k.leader) / 2;
+    const int cluster = int(blockIdx.x) / (2 * split), clusters = int(gridDim.x) / (2 * split);
+    const int steps = steps_of<P>(m, 0), k0 = steps * part / split, k1 = steps * (part + 1) / split;
+    Tiles<P> tiles(m, k.first, 0, clusters);
+    Tile t;
+    Loader<P> loader = loader_of<P>(maps, m, k);
+    Issuer<T, P> issuer = issuer_of<T, P>(m, k);
+    float *sums = reinterpret_cast<float *>(k.ring);  // [part][column][feature], once the ring is idle
+    uint32_t phase = 0;
+
+    for (int at = cluster; tiles.next(at, t); at += clusters) {
+        const int n = ceil_div(t.rows, kStepN) * kStepN, columns = n / split;  // columns that each pair adds up
+        const int feature = t.feature + int(k.rank) * (kTileFeatures<P> / 2);
+        if (warp == 0 && lane == 0) {
+            loader.load_tile(t, k0, k1);
+        } else if (warp == 1 && lane == 0 && k.rank == 0) {
+            if (issuer.run(t, sh.tmem, k0, k1)) mma_commit(smem_addr(&sh.tmem_full[0]), k.leader);
+        } else if (warp >= 4) {
+            mbar_wait(smem_addr(&sh.tmem_full[0]), phase, sh, m.status);
+        }
+        phase ^= 1;
+        __syncthreads();
+        const bool fine = !sh.aborted;
+        cluster_sync();  // every pair's products are over, and no load is under way
         fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        if (fine && warp >= 4) {
+            const int quarter = warp % 4, group = warp / 4 - 1;
+            for (int c = group * 8; c < n; c += 16) {
+                float v[8];
+                tmem_load(sh.tmem + (uint32_t(quarter * 32) << 16) + c, v);
+                const uint32_t to = map_to(smem_addr(sums), uint32_t(c / columns * 2) + k.rank) +
+                                    ((part * columns + c % columns) * kStagingRow + quarter * 32 + lane) * 4;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) store_cluster(to + j * kStagingRow * 4, v[j]);
+            }
+        }
+        fence_before();
+        cluster_sync();  // the sums are there
+        const int mine = min(columns, t.rows - part * columns);
+        if (fine) {
+            constexpr int kGroups = P == kUp ? 8 : 16;
+            for (int i = threadIdx.x; i < mine * kGroups; i += kThreads) {
+                const int column = i / kGroups, f = feature + i % kGroups * 8;
+                const int64_t row = t.first + part * columns + column;
+                if (f >= (P == kUp || P == kBack ? m.inner : m.hidden)) continue;
+                float a[8] = {}, b[8] = {}, g[8], u[8];
+                if constexpr (P == kBack) {
+                    load8(gu + row * 2 * m.inner + f, g);
+                    load8(gu + row * 2 * m.inner + m.inner + f, u);
+                }
+                for (int p = 0; p < split; ++p) {
+                    const float *from = sums + (p * columns + column) * kStagingRow + i % kGroups * 8;
+                    add8(from, a);
+                    if (P == kUp) add8(from + 64, b);
+                }
+                finish<T, P>(m, out, gu, row, f, a, b, g, u);
+            }
+        }
+        // The ring is the loads' again.
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
     }
+    if (threadIdx.x == 0) wait_previous();
+    tear_down(k);
 }
 
 // ---- launches ----------------------------------------------------------------------------------
@@ -758,7 +1013,7 @@ template <typename T> bool encode(CUtensorMap *map, const Dense &d) {
 }
 
 // Once per kernel and device: its shared memory.  The device's SM count in *sms.
-cudaError_t set_up(const void *kernel, int device, int index, int *sms) {
+cudaError_t prepare(const void *kernel, int device, int index, int *sms) {
     constexpr int kDevices = 64;
     static std::atomic<int> known_sms[kDevices];
     static std::atomic<uint32_t> done[kDevices];
@@ -774,6 +1029,20 @@ cudaError_t set_up(const void *kernel, int device, int index, int *sms) {
                                                int(shared_bytes(UGDR_X_EXPERTS_MAX)));
     if (e == cudaSuccess && kept) done[device].fetch_or(1u << index, std::memory_order_relaxed);
     return e;
+}
+
+// Pairs that share a tile: as many as keep every tile's pairs on the GPU at once, with four steps or
+// more for each.  What counts is known here from above only: a tile for each expert, or row if those
+// are fewer, and one for every kMaxN rows.
+template <Product P> int split_of(const ugdr_x_experts &m, int pairs) {
+    if (kWeightGrad<P>) return 1;
+    const int64_t row_tiles = (m.rows < uint64_t(m.nexp) ? int64_t(m.rows) : m.nexp) + int64_t(m.rows / kMaxN);
+    const int64_t features = P == kUp || P == kBack ? m.inner : m.hidden;
+    const int64_t tiles = row_tiles * ((features + kTileFeatures<P> - 1) / kTileFeatures<P>);
+    const int64_t depth = P == kDown ? m.inner : P == kInput ? 2 * int64_t(m.inner) : m.hidden;
+    for (int split = kMaxSplit; split > 1; split /= 2)
+        if (tiles * split <= pairs && depth >= 4 * split * kDepth) return split;
+    return 1;
 }
 
 // One product.  `a` and `b` are its operands: the weights and the rows, or the two row tensors of a
@@ -804,24 +1073,44 @@ cudaError_t launch(const ugdr_x_experts &m, const void *a, const void *b, void *
         db.box[db.rank - 1] = kWeightGrad<P> ? kDepth : kHalf >> i;
         if (!encode<T>(&maps.b[i], db)) return cudaErrorInvalidValue;
     }
+    // The most rows of B that a CTA can have to load per step, in whole boxes.
+    int load = kHalf;
+    if (!kWeightGrad<P> && m.rows < kMaxN) {
+        const int half = (int(m.rows) + kStepN - 1) / kStepN * kStepN / 2;
+        load = half == 16 ? 16 : (half + 31) / 32 * 32;
+    }
+    const uint32_t stage_bytes = kOperandBytes + uint32_t(load) * kDepth * 2;
+    const int stages = int(kRingBytes / stage_bytes) < kMaxStages ? int(kRingBytes / stage_bytes) : kMaxStages;
+    const Shape shape{m.counts, m.status, int(m.rows), m.nexp, m.hidden, m.inner, m.act, stages, stage_bytes};
 
-    auto *kernel = expert_kernel<T, P>;
     int device = 0, sms = 0;
     if (cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return e;
-    if (cudaError_t e = set_up(reinterpret_cast<const void *>(kernel), device, int(P) * 2 + std::is_same_v<T, __half>, &sms);
-        e != cudaSuccess)
-        return e;
-    cudaLaunchAttribute programmatic{};
-    programmatic.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    programmatic.val.programmaticStreamSerializationAllowed = 1;
+    auto *kernel = expert_kernel<T, P>;
+    constexpr int kIndex = int(P) * 2 + std::is_same_v<T, __half>;
+    if (cudaError_t e = prepare(reinterpret_cast<const void *>(kernel), device, kIndex, &sms); e != cudaSuccess) return e;
+    cudaLaunchAttribute attributes[2] = {};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(unsigned(sms / 2 * 2));
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = shared_bytes(m.nexp);
     config.stream = s;
-    config.attrs = &programmatic;
+    config.attrs = attributes;
     config.numAttrs = 1;
-    const Shape shape{m.counts, m.status, int(m.rows), m.nexp, m.hidden, m.inner, m.act};
+    if constexpr (!kWeightGrad<P>) {
+        const int split = split_of<P>(m, sms / 2);
+        if (split > 1) {
+            kernel = expert_split_kernel<T, P>;
+            if (cudaError_t e = prepare(reinterpret_cast<const void *>(kernel), device, 12 + kIndex, &sms);
+                e != cudaSuccess)
+                return e;
+            attributes[1].id = cudaLaunchAttributeClusterDimension;
+            attributes[1].val.clusterDim = {unsigned(2 * split), 1, 1};
+            config.gridDim = dim3(unsigned(sms / (2 * split) * (2 * split)));
+            config.numAttrs = 2;
+        }
+    }
     return cudaLaunchKernelEx(&config, kernel, maps, shape, static_cast<T *>(out), gu);
 }
 
