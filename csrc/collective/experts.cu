@@ -172,29 +172,32 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, u
                  : "memory");
 }
 
-// Operand descriptor for 128-byte swizzled tiles (rows of 128 bytes, atoms of 8 rows).  With the
+// Operand descriptors for 128-byte swizzled tiles (rows of 128 bytes, atoms of 8 rows).  With the
 // summed dimension inner, 8 features to an atom and 1024 bytes to the next 8.  With the features
 // inner, 64 of them to an atom of 8 summed positions, 1024 bytes to the next 8 positions and one
-// tile of 64 x 128 bytes to the next 64 features.  (Above its 18 bits an address names the CTA.)
-template <bool FEATURES_INNER> __device__ __forceinline__ uint64_t operand(uint32_t addr) {
-    const uint64_t leading = FEATURES_INNER ? kDepth * 128 / 16 : 1, stride = 1024 / 16;
-    return uint64_t(addr >> 4 & 0x3fff) | leading << 16 | stride << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+// tile of 64 x 128 bytes to the next 64 features.  The lower half begins with the address in units of
+// 16 bytes, to which offsets can be added.  (Above its 18 bits a shared address names the CTA.)
+template <bool FEATURES_INNER> __device__ __forceinline__ uint32_t operand(uint32_t addr) {
+    constexpr uint32_t kLeading = FEATURES_INNER ? kDepth * 128 / 16 : 1;
+    return (addr >> 4 & 0x3fff) | kLeading << 16;
 }
-// From one instruction's 16 summed positions to the next's, in the descriptor's address field.
-template <bool FEATURES_INNER> constexpr uint64_t kOperandStep = FEATURES_INNER ? 16 * 128 / 16 : 16 * 2 / 16;
+constexpr uint32_t kOperandUpper = 1024 / 16 | 1u << 14 | 2u << 29;  // stride, version, swizzle
+// From one instruction's 16 summed positions to the next's.
+template <bool FEATURES_INNER> constexpr uint32_t kOperandStep = FEATURES_INNER ? 16 * 128 / 16 : 16 * 2 / 16;
 
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-                 "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 a, b;\nsetp.ne.u32 p, %4, 0;\n"
+                 "mov.b64 a, {%1, %5};\nmov.b64 b, {%2, %5};\n"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, p;\n}" ::"r"(d),
+                 "r"(a), "r"(b), "r"(idesc), "r"(uint32_t(add)), "r"(kOperandUpper)
                  : "memory");
 }
-// Arrives on `bar` of both CTAs of the pair that begins at cluster rank `leader`, once the
-// instructions issued before are done.
-__device__ __forceinline__ void mma_commit(uint32_t bar, uint32_t leader) {
+// Arrives on `bar` of both CTAs of the pair, `mask` in the cluster, once the instructions issued
+// before are done.
+__device__ __forceinline__ void mma_commit(uint32_t bar, uint16_t mask) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
                      bar),
-                 "h"(uint16_t(3u << leader))
+                 "h"(mask)
                  : "memory");
 }
 // Programmatic launches: the next kernel of the stream may begin its set-up, and this one waits here
@@ -311,11 +314,15 @@ template <Product P> struct Tiles {
         }
         // Bands of kBand N tiles; inside, all N tiles of one feature tile before the next, so that
         // pairs that run together share weights and rows in the L2.
-        const int local = t - base, band = local / (kBand * mtiles), in_band = local - band * kBand * mtiles;
-        const int width = min(kBand, columns - band * kBand);
-        const int mtile = in_band / width, ntile = band * kBand + in_band - mtile * width;
+        int mtile = t - base, ntile = 0;
+        if (columns > 1) {
+            const int band = columns <= kBand ? 0 : mtile / (kBand * mtiles), width = min(kBand, columns - band * kBand);
+            const int in_band = mtile - band * kBand * mtiles;
+            mtile = in_band / width;
+            ntile = band * kBand + in_band - mtile * width;
+        }
         out.expert = expert;
-        out.part = P == kGradIn ? mtile / mparts : 0;
+        out.part = P == kGradIn ? mtile >= mparts : 0;
         out.feature = (mtile - out.part * mparts) * kTileFeatures<P>;
         if (kWeightGrad<P>) {
             out.first = first[expert];
@@ -438,7 +445,8 @@ struct Ring {
 
 // The thread that issues a CTA's loads.  Its loop is what a stage of few rows takes longest for, so
 // it is kept short: a loop of its own for every set of boxes, whose maps are then known.  (Picking
-// the map by an index made single rows per expert take 1.3 times as long.)
+// the map by an index made single rows per expert take 1.3 times as long.)  And what is not a loop
+// over the steps is there once only: instructions that a kernel meets first are read from memory.
 template <Product P> struct Loader {
     const Maps &maps;
     const Shape &m;
@@ -450,72 +458,67 @@ template <Product P> struct Loader {
 
     __device__ __forceinline__ bool wait() { return mbar_wait(empty + at.bar, at.parity, sh, m.status); }
 
-    // Steps [k0, k1) of a tile.
-    __device__ __forceinline__ bool load_tile(const Tile &t, int k0, int k1) {
-        if constexpr (kWeightGrad<P>) {
-            return load_steps<kHalf>(t, kHalf, k0, k1);
-        } else {
-            const int half = ceil_div(t.front(), kStepN) * kStepN / 2;
-            if (t.rows > kMaxN) return half > 96 ? load_wide<128>(t, half, k1) : load_wide<96>(t, half, k1);
-            return half > 96   ? load_steps<128>(t, half, k0, k1)
-                   : half > 64 ? load_steps<96>(t, half, k0, k1)
-                   : half > 32 ? load_steps<64>(t, half, k0, k1)
-                   : half > 16 ? load_steps<32>(t, half, k0, k1)
-                               : load_steps<16>(t, half, k0, k1);
-        }
-    }
-
-    // With LOAD of B's rows from this CTA's half on.
-    template <int LOAD> __device__ __forceinline__ bool load_steps(const Tile &t, int half, int k0, int k1) {
-        constexpr uint32_t kBytes = kOperandBytes + uint32_t(LOAD) * kDepth * 2;
-        int k = k0;
+    // Steps [k0, k1) of a tile; `then` in between, where the thread has time.
+    template <typename F> __device__ __forceinline__ bool load_tile(const Tile &t, int k0, int k1, F then) {
+        const int half = kWeightGrad<P> ? kHalf : ceil_div(t.front(), kStepN) * kStepN / 2;
+        const int load = half == 16 ? 16 : ceil_div(half, 32) * 32;  // rows of B from this CTA's half on
         if (!started) {
-            // The first steps: what does not come from the kernel before, then, once it is over, the rest.
-            const int filled = min(k1, k0 + m.stages);
-            const Ring begin = at;
-            for (; k < filled; ++k, at.next(m, stage0)) {
-                const uint32_t bar = barrier(t, k);
-                mbar_expect_cluster(bar, kBytes);
-                if (kEarlyA<P>) load_a(t, k, bar);
-                if (kEarlyB<P>) load_b<LOAD>(t, t.first, half, k, bar);
-            }
-            if (!kEarlyA<P> || !kEarlyB<P>) {
-                wait_previous();
-                at = begin;
-                for (k = k0; k < filled; ++k, at.next(m, stage0)) {
-                    const uint32_t bar = barrier(t, k);
-                    if (!kEarlyA<P>) load_a(t, k, bar);
-                    if (!kEarlyB<P>) load_b<LOAD>(t, t.first, half, k, bar);
-                }
-            }
+            k0 = load_first(t, half, load, k0, k1);
             started = true;
         }
-        for (; k < k1; ++k, at.next(m, stage0)) {
+        then();
+        if (kWeightGrad<P> || (load == 128 && t.rows <= kMaxN)) return load_steps<128>(t, half, k0, k1);
+        if (t.rows > kMaxN) return load_wide(t, half, k1);
+        return load == 96   ? load_steps<96>(t, half, k0, k1)
+               : load == 64 ? load_steps<64>(t, half, k0, k1)
+               : load == 32 ? load_steps<32>(t, half, k0, k1)
+                            : load_steps<16>(t, half, k0, k1);
+    }
+
+    // The kernel's first steps, as many as there are stages: what does not come from the kernel before,
+    // then, once that is over, the rest.  Returns the first step that is left.
+    __device__ __forceinline__ int load_first(const Tile &t, int half, int load, int k0, int k1) {
+        const int filled = !kWeightGrad<P> && t.rows > kMaxN ? k0 : min(k1, k0 + m.stages);
+        const Ring begin = at;
+        for (int k = k0; k < filled; ++k, at.next(m, stage0)) {
+            const uint32_t bar = barrier(t, k);
+            mbar_expect_cluster(bar, kOperandBytes + uint32_t(load) * kDepth * 2);
+            if (kEarlyA<P>) load_a(t, k, bar);
+            if (kEarlyB<P>) load_b(load, t, t.first, half, k, bar);
+        }
+        if (!kEarlyA<P> || !kEarlyB<P>) {
+            wait_previous();
+            at = begin;
+            for (int k = k0; k < filled; ++k, at.next(m, stage0)) {
+                const uint32_t bar = barrier(t, k);
+                if (!kEarlyA<P>) load_a(t, k, bar);
+                if (!kEarlyB<P>) load_b(load, t, t.first, half, k, bar);
+            }
+        }
+        return filled;
+    }
+
+    template <int LOAD> __device__ __forceinline__ bool load_steps(const Tile &t, int half, int k0, int k1) {
+        for (int k = k0; k < k1; ++k, at.next(m, stage0)) {
             if (!wait()) return false;
             const uint32_t bar = barrier(t, k);
-            mbar_expect_cluster(bar, kBytes);
+            mbar_expect_cluster(bar, kOperandBytes + uint32_t(LOAD) * kDepth * 2);
             load_a(t, k, bar);
-            load_b<LOAD>(t, t.first, half, k, bar);
+            load_b(LOAD, t, t.first, half, k, bar);
         }
         return true;
     }
 
     // A wide tile: a stage with the features and the first accumulator's rows, then one with the
     // second's rows.
-    template <int LOAD> __device__ __forceinline__ bool load_wide(const Tile &t, int half, int steps) {
-        if (!started) wait_previous();
-        started = true;
+    __device__ __forceinline__ bool load_wide(const Tile &t, int half, int steps) {
         const int front = t.front(), half2 = ceil_div(t.rows - front, kStepN) * kStepN / 2;
-        for (int k = 0; k < steps; ++k) {
+        for (int k = 0; k < 2 * steps; ++k, at.next(m, stage0)) {
             if (!wait()) return false;
-            mbar_expect_cluster(full + at.bar, kOperandBytes + uint32_t(LOAD) * kDepth * 2);
-            load_a(t, k, full + at.bar);
-            load_b<LOAD>(t, t.first, half, k, full + at.bar);
-            at.next(m, stage0);
-            if (!wait()) return false;
-            mbar_expect_cluster(full + at.bar, uint32_t(LOAD) * kDepth * 2);
-            load_b<LOAD>(t, t.first + front, half2, k, full + at.bar);
-            at.next(m, stage0);
+            const bool second = k & 1;
+            mbar_expect_cluster(full + at.bar, (second ? 1 : 2) * kOperandBytes);
+            if (!second) load_a(t, k / 2, full + at.bar);
+            load_b(kHalf, t, t.first + (second ? front : 0), second ? half2 : half, k / 2, full + at.bar);
         }
         return true;
     }
@@ -550,8 +553,7 @@ template <Product P> struct Loader {
         }
     }
 
-    template <int LOAD>
-    __device__ __forceinline__ void load_b(const Tile &t, int first, int half, int k, uint32_t bar) const {
+    __device__ __forceinline__ void load_b(int load, const Tile &t, int first, int half, int k, uint32_t bar) const {
         const uint32_t b = at.stage + kOperandBytes;
         const int depth = k * kDepth;
         if constexpr (kWeightGrad<P>) {
@@ -565,7 +567,7 @@ template <Product P> struct Loader {
 #pragma unroll
             for (int i = 0; i < kBoxes; ++i) {
                 constexpr int kFirst = kHalf;
-                if ((LOAD & kFirst >> i) == 0) continue;
+                if ((load & kFirst >> i) == 0) continue;
                 if constexpr (P == kInput)
                     tma_load(b + uint32_t(r) * kDepth * 2, &maps.b[i], bar, depth - part * part_steps * kDepth, part,
                              row + r);
@@ -579,9 +581,11 @@ template <Product P> struct Loader {
 
 // The thread that issues a pair's matrix instructions.
 template <typename T, Product P> struct Issuer {
+    static constexpr bool kInnerA = kFeaturesInner<P>, kInnerB = kWeightGrad<P>;
     const Shape &m;
     Shared &sh;
-    const uint32_t stage0, full, empty, leader;
+    const uint32_t stage0, full, empty;
+    const uint16_t mask;
     Ring at;
 
     __device__ __forceinline__ bool wait() {
@@ -589,18 +593,17 @@ template <typename T, Product P> struct Issuer {
         fence_after();
         return true;
     }
-    // One stage's products: A at `sa`, B at `sb`, `parts` times 16 deep.
+    // One stage's products: A in stage `sa`, B in stage `sb`, `parts` times 16 deep.
     __device__ __forceinline__ void multiply(uint32_t d, uint32_t sa, uint32_t sb, uint32_t idesc, int parts,
                                              bool add) const {
-        constexpr bool kInnerA = kFeaturesInner<P>, kInnerB = kWeightGrad<P>;
-        const uint64_t a = operand<kInnerA>(sa), b = operand<kInnerB>(sb);
+        const uint32_t a = operand<kInnerA>(sa), b = operand<kInnerB>(sb + kOperandBytes);
         for (int i = 0; i < parts; ++i)
             mma(d, a + i * kOperandStep<kInnerA>, b + i * kOperandStep<kInnerB>, idesc, add || i > 0);
     }
     // The instruction: its types, layouts and N.
     static __device__ __forceinline__ uint32_t instruction(int rows) {
         constexpr uint32_t kType = std::is_same_v<T, __nv_bfloat16> ? 1 : 0;
-        return 1u << 4 | kType << 7 | kType << 10 | uint32_t(kFeaturesInner<P>) << 15 | uint32_t(kWeightGrad<P>) << 16 |
+        return 1u << 4 | kType << 7 | kType << 10 | uint32_t(kInnerA) << 15 | uint32_t(kInnerB) << 16 |
                uint32_t(kPairFeatures / 16) << 24 | uint32_t(ceil_div(rows, kStepN) * (kStepN / 8)) << 17;
     }
 
@@ -611,8 +614,8 @@ template <typename T, Product P> struct Issuer {
             if (!wait()) return false;
             int parts = kDepth / 16;
             if (kWeightGrad<P>) parts = min(parts, ceil_div(t.rows - k * kDepth, 16));
-            multiply(d, at.stage, at.stage + kOperandBytes, idesc, parts, k > k0);
-            mma_commit(empty + at.bar, leader);
+            multiply(d, at.stage, at.stage, idesc, parts, k > k0);
+            mma_commit(empty + at.bar, mask);
         }
         return true;
     }
@@ -622,12 +625,12 @@ template <typename T, Product P> struct Issuer {
         for (int k = 0; k < steps; ++k, at.next(m, stage0)) {
             if (!wait()) return false;
             const uint32_t sa = at.stage, freed = empty + at.bar;
-            multiply(d, sa, sa + kOperandBytes, idesc, kDepth / 16, k > 0);
+            multiply(d, sa, sa, idesc, kDepth / 16, k > 0);
             at.next(m, stage0);
             if (!wait()) return false;
-            multiply(d2, sa, at.stage + kOperandBytes, idesc2, kDepth / 16, k > 0);
-            mma_commit(freed, leader);
-            mma_commit(empty + at.bar, leader);
+            multiply(d2, sa, at.stage, idesc2, kDepth / 16, k > 0);
+            mma_commit(freed, mask);
+            mma_commit(empty + at.bar, mask);
         }
         return true;
     }
@@ -688,7 +691,7 @@ struct Setup {
 template <Product P> __device__ __forceinline__ Setup set_up(const Maps &maps, const Shape &m) {
     extern __shared__ uint8_t raw[];
     Setup k;
-    k.ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);
+    k.ring = raw + (0u - smem_addr(raw)) % 1024;  // an offset, not a rounded pointer: accesses stay known to be shared
     k.staging = reinterpret_cast<float *>(k.ring + kRingBytes);
     k.sh = reinterpret_cast<Shared *>(reinterpret_cast<uint8_t *>(k.staging) + 2 * kStagingBytes);
     k.first = reinterpret_cast<int *>(k.sh + 1);
@@ -696,17 +699,15 @@ template <Product P> __device__ __forceinline__ Setup set_up(const Maps &maps, c
     k.rank = cta_rank() & 1;
     k.leader = cta_rank() - k.rank;
     Shared &sh = *k.sh;
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < kMaxStages; ++s) {
-            mbar_init(smem_addr(&sh.full[s]), 2);  // both CTAs' loads, counted in the leading CTA
-            mbar_init(smem_addr(&sh.empty[s]), 1);
-            mbar_init(smem_addr(&sh.tail[s]), 1);
+    if (threadIdx.x < kMaxStages) {
+        mbar_init(smem_addr(&sh.full[threadIdx.x]), 2);  // both CTAs' loads, counted in the leading CTA
+        mbar_init(smem_addr(&sh.empty[threadIdx.x]), 1);
+        mbar_init(smem_addr(&sh.tail[threadIdx.x]), 1);
+        if (threadIdx.x < 2) {
+            mbar_init(smem_addr(&sh.tmem_full[threadIdx.x]), 1);
+            mbar_init(smem_addr(&sh.tmem_empty[threadIdx.x]), 16);  // 8 epilogue warps of each CTA
         }
-        for (int s = 0; s < 2; ++s) {
-            mbar_init(smem_addr(&sh.tmem_full[s]), 1);
-            mbar_init(smem_addr(&sh.tmem_empty[s]), 16);  // 8 epilogue warps of each CTA
-        }
-        sh.aborted = sh.row_tiles = 0;
+        if (threadIdx.x == 0) sh.aborted = sh.row_tiles = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (threadIdx.x / 32 == 2) {
@@ -754,7 +755,8 @@ template <Product P> __device__ __forceinline__ Loader<P> loader_of(const Maps &
             {k.stage0, 0, 1}};  // parity 1: every stage is free
 }
 template <typename T, Product P> __device__ __forceinline__ Issuer<T, P> issuer_of(const Shape &m, const Setup &k) {
-    return {m, *k.sh, k.stage0, smem_addr(k.sh->full), smem_addr(k.sh->empty), k.leader, {k.stage0, 0, 0}};
+    return {m, *k.sh, k.stage0, smem_addr(k.sh->full), smem_addr(k.sh->empty), uint16_t(3u << k.leader),
+            {k.stage0, 0, 0}};
 }
 
 // One product, a pair of CTAs per tile.
@@ -770,8 +772,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
     if (warp == 0 && lane == 0) {
         Loader<P> loader = loader_of<P>(maps, m, k);
-        for (int at = pair; tiles.next(at, t); at += pairs)
-            if (!loader.load_tile(t, 0, steps_of<P>(m, t.rows))) break;
+        bool more = tiles.next(pair, t);
+        for (int at = pair + pairs; more; at += pairs) {
+            const Tile u = t;
+            const int steps = steps_of<P>(m, u.rows);
+            auto then = [&] { more = tiles.next(at, t); };
+            if (steps == 0)
+                then();
+            else if (!loader.load_tile(u, 0, steps, then))
+                break;
+        }
         wait_previous();  // in any case: a kernel is over only when those before it are
     } else if (warp == 1 && lane == 0 && k.rank == 0) {
         Issuer<T, P> issuer = issuer_of<T, P>(m, k);
@@ -787,8 +797,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const bool wide = !kWeightGrad<P> && t.rows > kMaxN;
             if (!wait_accumulator(acc) || (wide && !wait_accumulator(acc + 1))) break;
             if (!(wide ? issuer.run_wide(t, d, d2, steps) : issuer.run(t, d, 0, steps))) break;
-            mma_commit(smem_addr(&sh.tmem_full[acc++ & 1]), k.leader);
-            if (wide) mma_commit(smem_addr(&sh.tmem_full[acc++ & 1]), k.leader);
+            mma_commit(smem_addr(&sh.tmem_full[acc++ & 1]), issuer.mask);
+            if (wide) mma_commit(smem_addr(&sh.tmem_full[acc++ & 1]), issuer.mask);
         }
     } else if (warp == 2 && kWeightGrad<P>) {
         // Tails: the rows behind the group in its last step, up to the next 16, become zeros.
@@ -921,9 +931,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n = ceil_div(t.rows, kStepN) * kStepN, columns = n / split;  // columns that each pair adds up
         const int feature = t.feature + int(k.rank) * (kTileFeatures<P> / 2);
         if (warp == 0 && lane == 0) {
-            loader.load_tile(t, k0, k1);
+            loader.load_tile(t, k0, k1, [] {});
         } else if (warp == 1 && lane == 0 && k.rank == 0) {
-            if (issuer.run(t, sh.tmem, k0, k1)) mma_commit(smem_addr(&sh.tmem_full[0]), k.leader);
+            if (issuer.run(t, sh.tmem, k0, k1)) mma_commit(smem_addr(&sh.tmem_full[0]), issuer.mask);
         } else if (warp >= 4) {
             mbar_wait(smem_addr(&sh.tmem_full[0]), phase, sh, m.status);
         }
