@@ -75,7 +75,6 @@ struct Shared {
     alignas(8) uint64_t full[kMaxStages], empty[kMaxStages], tail[kMaxStages], tmem_full[2], tmem_empty[2];
     uint32_t tmem;
     int aborted;
-    int row_tiles;  // of all experts, at most kMaxN rows each
     long long scan[kThreads / 32];
 };
 constexpr size_t shared_bytes(int nexp) {
@@ -251,11 +250,6 @@ struct Tile {
     int first;    // rows products: the tile's first row.  Weight gradients: the group's
     int rows;     // likewise, of the tile or the group
     int column;   // weight gradients: first of the N
-
-    // Rows that the tile's first accumulator takes; a wide tile's second one takes the others.
-    __device__ __forceinline__ int front() const {
-        return rows <= kMaxN ? rows : ceil_div(ceil_div(rows, 2), kStepN) * kStepN;
-    }
 };
 
 // Features of a tile of the pair: with kUp 128 of the gate and the same 128 of the up projection.
@@ -268,48 +262,29 @@ template <Product P> __device__ __forceinline__ int steps_of(const Shape &m, int
 }
 
 // Walks the tile list in order: next() finds tile t for increasing t.
+//
+// An expert's rows are cut into tiles of about the same size, all but the last a multiple of kStepN.
+// (Tiles of up to 512 rows, in both accumulators, load the features once for more rows; they gained
+// 4 % at 300 rows per expert and cost 1 to 4 % elsewhere, for the longer code and the accumulators
+// that no products run beside.)
 template <Product P> struct Tiles {
     const int *first;  // first row of each expert's group, and the end of the last
-    int nexp, mtiles, mparts, ntiles, steps;
-    bool wide;
+    int nexp, mtiles, mparts, ntiles;
     int expert = -1, base = 0, size = 0, n = 0, columns = 0, per = 0;
 
-    // `workers`: pairs (or clusters) that share the list.
-    __device__ Tiles(const Shape &m, const int *first_, int row_tiles, int workers) : first(first_), nexp(m.nexp) {
+    __device__ Tiles(const Shape &m, const int *first_) : first(first_), nexp(m.nexp) {
         const int features = P == kUp || P == kBack || P == kGradIn ? m.inner : m.hidden;
         mparts = ceil_div(features, kTileFeatures<P>);
         mtiles = P == kGradIn ? 2 * mparts : mparts;
         ntiles = P == kGradOut ? ceil_div(m.inner, kMaxN) : P == kGradIn ? ceil_div(m.hidden, kMaxN) : 0;
-        steps = kWeightGrad<P> ? 0 : steps_of<P>(m, 0);
-        // Wide tiles leave work for fewer pairs: only where there is plenty.
-        wide = !kWeightGrad<P> && m.stage_bytes == 2 * kOperandBytes && int64_t(row_tiles) * mtiles >= 4 * workers;
-    }
-    // How the expert's rows are cut into tiles: of about the same size, all but the last a multiple
-    // of kStepN.  Clocks of a step: 2 per row for the products, and 64 bytes per clock for loading,
-    // which is 256 for the features and 1 per row.  So two tiles of 160 rows would wait for their
-    // loads, and one wide tile of 288, which loads the features once and fills the accumulators of
-    // two, is faster (32 experts of 300 rows, 7168 x 2048: 0.87 ms with tiles of at most 256 rows,
-    // 0.69 with wide ones), as long as its many steps outweigh that its accumulators, some 32 clocks
-    // per row, are moved out while no products run.
-    __device__ __forceinline__ void cut() {
-        columns = ceil_div(n, kMaxN);
-        per = columns == 0 ? 0 : ceil_div(ceil_div(n, columns), kStepN) * kStepN;
-        if (!wide || columns < 2) return;
-        const int wcolumns = ceil_div(n, 2 * kMaxN), wper = ceil_div(ceil_div(n, wcolumns), kStepN) * kStepN;
-        if (wper <= kMaxN) return;
-        const int64_t cost = int64_t(columns) * max(2 * per, 256 + per);
-        const int64_t wcost = int64_t(wcolumns) * (max(2 * wper, 256 + wper) + 32 * wper / steps);
-        if (wcost < cost) columns = wcolumns, per = wper;
     }
     __device__ __forceinline__ bool next(int t, Tile &out) {
         while (t >= base + size) {
             if (++expert >= nexp) return false;
             base += size;
             n = first[expert + 1] - first[expert];
-            if (kWeightGrad<P>)
-                columns = ntiles;
-            else
-                cut();
+            columns = kWeightGrad<P> ? ntiles : ceil_div(n, kMaxN);
+            if (columns > 0) per = ceil_div(ceil_div(n, columns), kStepN) * kStepN;
             size = mtiles * columns;
         }
         // Bands of kBand N tiles; inside, all N tiles of one feature tile before the next, so that
@@ -363,14 +338,11 @@ __device__ void scan_counts(const Shape &m, Shared &sh, int *first) {
     __syncthreads();
     for (int w = 0; w < warp; ++w) upto += sh.scan[w];
     long long at = upto - own;
-    int row_tiles = 0;
     for (int e = e0; e < e1; ++e) {
         const int c = first[e];
         first[e] = int(min(at, (long long)m.rows));
         at += c;
-        row_tiles += ceil_div(int(min(at, (long long)m.rows)) - first[e], kMaxN);
     }
-    if (row_tiles > 0) atomicAdd(&sh.row_tiles, row_tiles);
     if (threadIdx.x == kThreads - 1) {
         first[m.nexp] = int(min(upto, (long long)m.rows));
         bad |= upto > m.rows;
@@ -458,17 +430,15 @@ template <Product P> struct Loader {
 
     __device__ __forceinline__ bool wait() { return mbar_wait(empty + at.bar, at.parity, sh, m.status); }
 
-    // Steps [k0, k1) of a tile; `then` in between, where the thread has time.
-    template <typename F> __device__ __forceinline__ bool load_tile(const Tile &t, int k0, int k1, F then) {
-        const int half = kWeightGrad<P> ? kHalf : ceil_div(t.front(), kStepN) * kStepN / 2;
+    // Steps [k0, k1) of a tile.
+    __device__ __forceinline__ bool load_tile(const Tile &t, int k0, int k1) {
+        const int half = kWeightGrad<P> ? kHalf : ceil_div(t.rows, kStepN) * kStepN / 2;
         const int load = half == 16 ? 16 : ceil_div(half, 32) * 32;  // rows of B from this CTA's half on
         if (!started) {
             k0 = load_first(t, half, load, k0, k1);
             started = true;
         }
-        then();
-        if (kWeightGrad<P> || (load == 128 && t.rows <= kMaxN)) return load_steps<128>(t, half, k0, k1);
-        if (t.rows > kMaxN) return load_wide(t, half, k1);
+        if (kWeightGrad<P> || load == 128) return load_steps<128>(t, half, k0, k1);
         return load == 96   ? load_steps<96>(t, half, k0, k1)
                : load == 64 ? load_steps<64>(t, half, k0, k1)
                : load == 32 ? load_steps<32>(t, half, k0, k1)
@@ -478,13 +448,13 @@ template <Product P> struct Loader {
     // The kernel's first steps, as many as there are stages: what does not come from the kernel before,
     // then, once that is over, the rest.  Returns the first step that is left.
     __device__ __forceinline__ int load_first(const Tile &t, int half, int load, int k0, int k1) {
-        const int filled = !kWeightGrad<P> && t.rows > kMaxN ? k0 : min(k1, k0 + m.stages);
+        const int filled = min(k1, k0 + m.stages);
         const Ring begin = at;
         for (int k = k0; k < filled; ++k, at.next(m, stage0)) {
             const uint32_t bar = barrier(t, k);
             mbar_expect_cluster(bar, kOperandBytes + uint32_t(load) * kDepth * 2);
             if (kEarlyA<P>) load_a(t, k, bar);
-            if (kEarlyB<P>) load_b(load, t, t.first, half, k, bar);
+            if (kEarlyB<P>) load_b(load, t, half, k, bar);
         }
         if (!kEarlyA<P> || !kEarlyB<P>) {
             wait_previous();
@@ -492,7 +462,7 @@ template <Product P> struct Loader {
             for (int k = k0; k < filled; ++k, at.next(m, stage0)) {
                 const uint32_t bar = barrier(t, k);
                 if (!kEarlyA<P>) load_a(t, k, bar);
-                if (!kEarlyB<P>) load_b(load, t, t.first, half, k, bar);
+                if (!kEarlyB<P>) load_b(load, t, half, k, bar);
             }
         }
         return filled;
@@ -504,21 +474,7 @@ template <Product P> struct Loader {
             const uint32_t bar = barrier(t, k);
             mbar_expect_cluster(bar, kOperandBytes + uint32_t(LOAD) * kDepth * 2);
             load_a(t, k, bar);
-            load_b(LOAD, t, t.first, half, k, bar);
-        }
-        return true;
-    }
-
-    // A wide tile: a stage with the features and the first accumulator's rows, then one with the
-    // second's rows.
-    __device__ __forceinline__ bool load_wide(const Tile &t, int half, int steps) {
-        const int front = t.front(), half2 = ceil_div(t.rows - front, kStepN) * kStepN / 2;
-        for (int k = 0; k < 2 * steps; ++k, at.next(m, stage0)) {
-            if (!wait()) return false;
-            const bool second = k & 1;
-            mbar_expect_cluster(full + at.bar, (second ? 1 : 2) * kOperandBytes);
-            if (!second) load_a(t, k / 2, full + at.bar);
-            load_b(kHalf, t, t.first + (second ? front : 0), second ? half2 : half, k / 2, full + at.bar);
+            load_b(LOAD, t, half, k, bar);
         }
         return true;
     }
@@ -553,7 +509,7 @@ template <Product P> struct Loader {
         }
     }
 
-    __device__ __forceinline__ void load_b(int load, const Tile &t, int first, int half, int k, uint32_t bar) const {
+    __device__ __forceinline__ void load_b(int load, const Tile &t, int half, int k, uint32_t bar) const {
         const uint32_t b = at.stage + kOperandBytes;
         const int depth = k * kDepth;
         if constexpr (kWeightGrad<P>) {
@@ -562,7 +518,7 @@ template <Product P> struct Loader {
                 tma_load(b + uint32_t(c) * kOperandBytes / 2, &maps.b[0], bar, t.column + int(rank) * kHalf + c * 64,
                          t.first + depth);
         } else {
-            const int row = first + int(rank) * half, part = P == kInput ? k >= part_steps : 0;
+            const int row = t.first + int(rank) * half, part = P == kInput ? k >= part_steps : 0;
             int r = 0;
 #pragma unroll
             for (int i = 0; i < kBoxes; ++i) {
@@ -593,12 +549,12 @@ template <typename T, Product P> struct Issuer {
         fence_after();
         return true;
     }
-    // One stage's products: A in stage `sa`, B in stage `sb`, `parts` times 16 deep.
-    __device__ __forceinline__ void multiply(uint32_t d, uint32_t sa, uint32_t sb, uint32_t idesc, int parts,
-                                             bool add) const {
-        const uint32_t a = operand<kInnerA>(sa), b = operand<kInnerB>(sb + kOperandBytes);
-        for (int i = 0; i < parts; ++i)
-            mma(d, a + i * kOperandStep<kInnerA>, b + i * kOperandStep<kInnerB>, idesc, add || i > 0);
+    // The products of the current stage, `parts` times 16 deep.
+    __device__ __forceinline__ void multiply(uint32_t d, uint32_t idesc, int parts, bool add) const {
+        const uint32_t a = operand<kInnerA>(at.stage), b = operand<kInnerB>(at.stage + kOperandBytes);
+#pragma unroll
+        for (int i = 0; i < kDepth / 16; ++i)
+            if (i < parts) mma(d, a + i * kOperandStep<kInnerA>, b + i * kOperandStep<kInnerB>, idesc, add || i > 0);
     }
     // The instruction: its types, layouts and N.
     static __device__ __forceinline__ uint32_t instruction(int rows) {
@@ -614,22 +570,7 @@ template <typename T, Product P> struct Issuer {
             if (!wait()) return false;
             int parts = kDepth / 16;
             if (kWeightGrad<P>) parts = min(parts, ceil_div(t.rows - k * kDepth, 16));
-            multiply(d, at.stage, at.stage, idesc, parts, k > k0);
-            mma_commit(empty + at.bar, mask);
-        }
-        return true;
-    }
-    // A wide tile into the accumulators at d and d2.
-    __device__ __forceinline__ bool run_wide(const Tile &t, uint32_t d, uint32_t d2, int steps) {
-        const uint32_t idesc = instruction(t.front()), idesc2 = instruction(t.rows - t.front());
-        for (int k = 0; k < steps; ++k, at.next(m, stage0)) {
-            if (!wait()) return false;
-            const uint32_t sa = at.stage, freed = empty + at.bar;
-            multiply(d, sa, sa, idesc, kDepth / 16, k > 0);
-            at.next(m, stage0);
-            if (!wait()) return false;
-            multiply(d2, sa, at.stage, idesc2, kDepth / 16, k > 0);
-            mma_commit(freed, mask);
+            multiply(d, idesc, parts, k > k0);
             mma_commit(empty + at.bar, mask);
         }
         return true;
@@ -707,7 +648,7 @@ template <Product P> __device__ __forceinline__ Setup set_up(const Maps &maps, c
             mbar_init(smem_addr(&sh.tmem_full[threadIdx.x]), 1);
             mbar_init(smem_addr(&sh.tmem_empty[threadIdx.x]), 16);  // 8 epilogue warps of each CTA
         }
-        if (threadIdx.x == 0) sh.aborted = sh.row_tiles = 0;
+        if (threadIdx.x == 0) sh.aborted = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (threadIdx.x / 32 == 2) {
@@ -766,39 +707,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const Setup k = set_up<P>(maps, m);
     Shared &sh = *k.sh;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, pair = blockIdx.x / 2, pairs = gridDim.x / 2;
-    Tiles<P> tiles(m, k.first, sh.row_tiles, pairs);
+    Tiles<P> tiles(m, k.first);
     Tile t;
     uint32_t acc = 0;  // accumulators used so far: they take turns
 
     if (warp == 0 && lane == 0) {
         Loader<P> loader = loader_of<P>(maps, m, k);
-        bool more = tiles.next(pair, t);
-        for (int at = pair + pairs; more; at += pairs) {
-            const Tile u = t;
-            const int steps = steps_of<P>(m, u.rows);
-            auto then = [&] { more = tiles.next(at, t); };
-            if (steps == 0)
-                then();
-            else if (!loader.load_tile(u, 0, steps, then))
-                break;
-        }
+        for (int at = pair; tiles.next(at, t); at += pairs)
+            if (!loader.load_tile(t, 0, steps_of<P>(m, t.rows))) break;
         wait_previous();  // in any case: a kernel is over only when those before it are
     } else if (warp == 1 && lane == 0 && k.rank == 0) {
         Issuer<T, P> issuer = issuer_of<T, P>(m, k);
-        auto wait_accumulator = [&](uint32_t a) {
-            if (!mbar_wait(smem_addr(&sh.tmem_empty[a & 1]), (a / 2 + 1) & 1, sh, m.status)) return false;
-            fence_after();
-            return true;
-        };
         for (int at = pair; tiles.next(at, t); at += pairs) {
             const int steps = steps_of<P>(m, t.rows);
             if (steps == 0) continue;
-            const uint32_t d = sh.tmem + (acc & 1) * kMaxN, d2 = sh.tmem + (~acc & 1) * kMaxN;
-            const bool wide = !kWeightGrad<P> && t.rows > kMaxN;
-            if (!wait_accumulator(acc) || (wide && !wait_accumulator(acc + 1))) break;
-            if (!(wide ? issuer.run_wide(t, d, d2, steps) : issuer.run(t, d, 0, steps))) break;
-            mma_commit(smem_addr(&sh.tmem_full[acc++ & 1]), issuer.mask);
-            if (wide) mma_commit(smem_addr(&sh.tmem_full[acc++ & 1]), issuer.mask);
+            if (!mbar_wait(smem_addr(&sh.tmem_empty[acc & 1]), (acc / 2 + 1) & 1, sh, m.status)) break;
+            fence_after();
+            if (!issuer.run(t, sh.tmem + (acc & 1) * kMaxN, 0, steps)) break;
+            mma_commit(smem_addr(&sh.tmem_full[acc & 1]), issuer.mask);
+            ++acc;
         }
     } else if (warp == 2 && kWeightGrad<P>) {
         // Tails: the rows behind the group in its last step, up to the next 16, become zeros.
@@ -826,82 +753,76 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         // group of four warps takes every other chunk of columns.
         const int quarter = warp % 4, group = warp / 4 - 1;
         const uint32_t lanes = sh.tmem + (uint32_t(quarter * 32) << 16), empty = map_to(smem_addr(sh.tmem_empty), k.leader);
-        bool go = true;
-        for (int at = pair; go && tiles.next(at, t); at += pairs) {
+        for (int at = pair; tiles.next(at, t); at += pairs) {
             const bool none = steps_of<P>(m, t.rows) == 0;
             const int feature = t.feature + int(k.rank) * (kTileFeatures<P> / 2);
-            const int front = kWeightGrad<P> ? t.rows : t.front();
-            int from = 0;
-            do {  // once, or for both accumulators of a wide tile
-                if (!none) {
-                    const bool full = mbar_wait(smem_addr(&sh.tmem_full[acc & 1]), (acc / 2) & 1, sh, m.status);
-                    if (!(go = group_all(group, full))) break;
-                    fence_after();
-                }
-                const uint32_t columns = lanes + (acc & 1) * kMaxN;
-                if constexpr (kWeightGrad<P>) {
-                    // A thread has one row of the gradient and writes its columns.
-                    const int width = P == kGradOut ? m.inner : m.hidden, height = P == kGradOut ? m.hidden : m.inner;
-                    const int f = feature + quarter * 32 + lane;
-                    T *row = out + ((int64_t(t.expert) * (P == kGradIn ? 2 : 1) + t.part) * height + f) * width + t.column;
-                    for (int c = group * kChunk; c < kMaxN; c += 2 * kChunk) {
-                        float v[kChunk];
-                        if (none) {
+            if (!none) {
+                if (!group_all(group, mbar_wait(smem_addr(&sh.tmem_full[acc & 1]), (acc / 2) & 1, sh, m.status)))
+                    break;
+                fence_after();
+            }
+            const uint32_t columns = lanes + (acc & 1) * kMaxN;
+            if constexpr (kWeightGrad<P>) {
+                // A thread has one row of the gradient and writes its columns.
+                const int width = P == kGradOut ? m.inner : m.hidden, height = P == kGradOut ? m.hidden : m.inner;
+                const int f = feature + quarter * 32 + lane;
+                T *row = out + ((int64_t(t.expert) * (P == kGradIn ? 2 : 1) + t.part) * height + f) * width + t.column;
+                for (int c = group * kChunk; c < kMaxN; c += 2 * kChunk) {
+                    float v[kChunk];
+                    if (none) {
 #pragma unroll
-                            for (int j = 0; j < kChunk; ++j) v[j] = 0.f;
-                        } else {
-                            tmem_load(columns + c, v);
-                        }
-                        if (f < height) {
-#pragma unroll
-                            for (int j = 0; j < kChunk; j += 8)
-                                if (t.column + c + j < width) store8(row + c + j, v + j);
-                        }
+                        for (int j = 0; j < kChunk; ++j) v[j] = 0.f;
+                    } else {
+                        tmem_load(columns + c, v);
                     }
-                } else {
-                    // A chunk of rows at a time, turned around in shared memory: then 8 lanes hold 64
-                    // of a row's features, 8 next to each other per lane.
-                    const int rows = from == 0 ? front : t.rows - front, r = quarter * 4 + lane / 8;
-                    float *buffer = k.staging + group * (kStagingBytes / 4);
-                    for (int c = group * kChunk; c < rows; c += 2 * kChunk) {
-                        const int64_t row = t.first + from + c + r;
-                        float g[2][8], u[2][8];
-                        if constexpr (P == kBack) {  // under way while the accumulators are turned around
+                    if (f < height) {
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const int f = feature + i * 64 + lane % 8 * 8;
-                                if (c + r < rows && f < m.inner) {
-                                    load8(gu + row * 2 * m.inner + f, g[i]);
-                                    load8(gu + row * 2 * m.inner + m.inner + f, u[i]);
-                                }
+                        for (int j = 0; j < kChunk; j += 8)
+                            if (t.column + c + j < width) store8(row + c + j, v + j);
+                    }
+                }
+            } else {
+                // A chunk of rows at a time, turned around in shared memory: then 8 lanes hold 64
+                // of a row's features, 8 next to each other per lane.
+                const int r = quarter * 4 + lane / 8;
+                float *buffer = k.staging + group * (kStagingBytes / 4);
+                for (int c = group * kChunk; c < t.rows; c += 2 * kChunk) {
+                    const int64_t row = t.first + c + r;
+                    float g[2][8], u[2][8];
+                    if constexpr (P == kBack) {  // under way while the accumulators are turned around
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int f = feature + i * 64 + lane % 8 * 8;
+                            if (c + r < t.rows && f < m.inner) {
+                                load8(gu + row * 2 * m.inner + f, g[i]);
+                                load8(gu + row * 2 * m.inner + m.inner + f, u[i]);
                             }
                         }
-                        float v[kChunk];
-                        tmem_load(columns + c, v);
-#pragma unroll
-                        for (int j = 0; j < kChunk; ++j) buffer[j * kStagingRow + quarter * 32 + lane] = v[j];
-                        group_sync(group);
-                        const float *sums = buffer + r * kStagingRow + lane % 8 * 8;
-#pragma unroll
-                        for (int i = 0; i < (P == kUp ? 1 : 2); ++i) {
-                            const int f = feature + i * 64 + lane % 8 * 8;
-                            if (c + r >= rows || f >= (P == kUp || P == kBack ? m.inner : m.hidden)) continue;
-                            float a[8], b[8];
-                            load8(sums + i * 64, a);
-                            if (P == kUp) load8(sums + 64, b);
-                            finish<T, P>(m, out, gu, row, f, a, b, g[i], u[i]);
-                        }
-                        group_sync(group);  // the buffer is free again
                     }
+                    float v[kChunk];
+                    tmem_load(columns + c, v);
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) buffer[j * kStagingRow + quarter * 32 + lane] = v[j];
+                    group_sync(group);
+                    const float *sums = buffer + r * kStagingRow + lane % 8 * 8;
+#pragma unroll
+                    for (int i = 0; i < (P == kUp ? 1 : 2); ++i) {
+                        const int f = feature + i * 64 + lane % 8 * 8;
+                        if (c + r >= t.rows || f >= (P == kUp || P == kBack ? m.inner : m.hidden)) continue;
+                        float a[8], b[8];
+                        load8(sums + i * 64, a);
+                        if (P == kUp) load8(sums + 64, b);
+                        finish<T, P>(m, out, gu, row, f, a, b, g[i], u[i]);
+                    }
+                    group_sync(group);  // the buffer is free again
                 }
-                if (!none) {
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(empty + (acc & 1) * 8);
-                    ++acc;
-                }
-                from += front;
-            } while (!kWeightGrad<P> && from < t.rows);
+            }
+            if (!none) {
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(empty + (acc & 1) * 8);
+                ++acc;
+            }
         }
     }
     tear_down(k);
@@ -920,7 +841,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int split = int(cluster_size()) / 2, part = int(k.leader) / 2;
     const int cluster = int(blockIdx.x) / (2 * split), clusters = int(gridDim.x) / (2 * split);
     const int steps = steps_of<P>(m, 0), k0 = steps * part / split, k1 = steps * (part + 1) / split;
-    Tiles<P> tiles(m, k.first, 0, clusters);
+    Tiles<P> tiles(m, k.first);
     Tile t;
     Loader<P> loader = loader_of<P>(maps, m, k);
     Issuer<T, P> issuer = issuer_of<T, P>(m, k);
@@ -931,7 +852,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n = ceil_div(t.rows, kStepN) * kStepN, columns = n / split;  // columns that each pair adds up
         const int feature = t.feature + int(k.rank) * (kTileFeatures<P> / 2);
         if (warp == 0 && lane == 0) {
-            loader.load_tile(t, k0, k1, [] {});
+            loader.load_tile(t, k0, k1);
         } else if (warp == 1 && lane == 0 && k.rank == 0) {
             if (issuer.run(t, sh.tmem, k0, k1)) mma_commit(smem_addr(&sh.tmem_full[0]), issuer.mask);
         } else if (warp >= 4) {
