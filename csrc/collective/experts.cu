@@ -656,8 +656,7 @@ template <Product P> __device__ __forceinline__ Setup set_up(const Maps &maps, c
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
-    if (threadIdx.x >= 32 && threadIdx.x < 32 + 1 + (kWeightGrad<P> ? 1 : kBoxes))
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a + (threadIdx.x - 32)) : "memory");
+    if (threadIdx.x == 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a) : "memory");
     fence_before();
     cluster_sync();
     fence_after();
@@ -998,12 +997,6 @@ cudaError_t launch(const ugdr_x_experts &m, const void *a, const void *b, void *
         db = {b, 3, {F, 2, R}, {64, 1, 0}};
     else
         db = {b, 2, {P == kUp || P == kBack || P == kGradIn ? H : F, R}, {64, 0}};
-    Maps maps;
-    if (!encode<T>(&maps.a, da)) return cudaErrorInvalidValue;
-    for (int i = 0; i < (kWeightGrad<P> ? 1 : kBoxes); ++i) {
-        db.box[db.rank - 1] = kWeightGrad<P> ? kDepth : kHalf >> i;
-        if (!encode<T>(&maps.b[i], db)) return cudaErrorInvalidValue;
-    }
     // The most rows of B that a CTA can have to load per step, in whole boxes.
     int load = kHalf;
     if (!kWeightGrad<P> && m.rows < kMaxN) {
@@ -1012,6 +1005,13 @@ cudaError_t launch(const ugdr_x_experts &m, const void *a, const void *b, void *
     }
     const uint32_t stage_bytes = kOperandBytes + uint32_t(load) * kDepth * 2;
     const int stages = int(kRingBytes / stage_bytes) < kMaxStages ? int(kRingBytes / stage_bytes) : kMaxStages;
+    Maps maps;
+    if (!encode<T>(&maps.a, da)) return cudaErrorInvalidValue;
+    for (int i = 0; i < (kWeightGrad<P> ? 1 : kBoxes); ++i) {
+        if (kHalf >> i > load) continue;  // too large ever to be asked for
+        db.box[db.rank - 1] = kWeightGrad<P> ? kDepth : kHalf >> i;
+        if (!encode<T>(&maps.b[i], db)) return cudaErrorInvalidValue;
+    }
     const Shape shape{m.counts, m.status, int(m.rows), m.nexp, m.hidden, m.inner, m.act, stages, stage_bytes};
 
     int device = 0, sms = 0;

@@ -116,17 +116,22 @@ def check_status(device: torch.device | int | None = None) -> None:
                             2: "expert counts are negative or exceed the rows"}.get(st, f"status {st}"))
 
 
-def _rows(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor, dtype: torch.dtype | None = None) -> None:
+def _rows(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor, dtype: torch.dtype | None = None
+          ) -> tuple[int, int]:
+    """The addresses that t begins and ends at, checked to be a dense tensor of that shape beside `like`."""
     dtype = dtype or like.dtype
-    if not isinstance(t, torch.Tensor) or t.device != like.device or t.dtype != dtype:
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != like.device:
         raise ValueError(f"{name} must be a {dtype} tensor on {like.device}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
-    if not t.is_contiguous() or t.data_ptr() % 16:
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    at = t.data_ptr()
+    if at % 16 or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous and 16-byte aligned")
+    return at, at + t.nbytes
 
 
-def _checked(x, counts, w_in, w_out, act: str) -> _Experts:
+def _checked(x, counts, w_in, w_out, act: str) -> tuple[_Experts, dict[str, tuple[int, int]]]:
+    """The call's description, and the addresses that its inputs begin and end at."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _TYPES or x.dim() != 2:
         raise ValueError("x must be a CUDA tensor [rows, hidden] of bfloat16 or float16")
     if act not in _ACTS:
@@ -135,7 +140,7 @@ def _checked(x, counts, w_in, w_out, act: str) -> _Experts:
     if not isinstance(counts, torch.Tensor) or counts.dtype != torch.int32 or counts.dim() != 1 \
             or counts.device != x.device or not counts.is_contiguous():
         raise ValueError(f"counts must be a contiguous int32 tensor [experts] on {x.device}")
-    nexp = counts.numel()
+    nexp = counts.shape[0]
     if not 1 <= nexp <= MAX_EXPERTS:
         raise ValueError(f"1..{MAX_EXPERTS} experts supported, got {nexp}")
     if not isinstance(w_out, torch.Tensor) or w_out.dim() != 3:
@@ -145,37 +150,32 @@ def _checked(x, counts, w_in, w_out, act: str) -> _Experts:
         raise ValueError(f"hidden and inner must be multiples of 8, got {hidden} and {inner}")
     if rows >= 1 << 31:
         raise ValueError(f"at most 2**31 - 1 rows, got {rows}")
-    _rows(x, "x", (rows, hidden), x)
-    _rows(w_in, "w_in", (nexp, 2, inner, hidden), x)
-    _rows(w_out, "w_out", (nexp, hidden, inner), x)
-    return _Experts(counts.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), None, rows, nexp, hidden, inner,
-                    _TYPES[x.dtype], _ACTS[act])
+    at = counts.data_ptr()
+    spans = {"x": _rows(x, "x", (rows, hidden), x), "counts": (at, at + 4 * nexp),
+             "w_in": _rows(w_in, "w_in", (nexp, 2, inner, hidden), x),
+             "w_out": _rows(w_out, "w_out", (nexp, hidden, inner), x)}
+    return _Experts(at, spans["w_in"][0], spans["w_out"][0], None, rows, nexp, hidden, inner, _TYPES[x.dtype],
+                    _ACTS[act]), spans
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    a0, b0 = a.data_ptr(), b.data_ptr()
-    return a0 < b0 + b.numel() * b.element_size() and b0 < a0 + a.numel() * a.element_size()
-
-
-def _apart(out: torch.Tensor, name: str, inputs: dict, same: tuple = ()) -> None:
-    """`out` overlaps none of the inputs; those named in `same` it may be as a whole."""
-    for other, t in inputs.items():
-        if _overlap(out, t) and not (other in same and out.data_ptr() == t.data_ptr()):
+def _apart(name: str, span: tuple[int, int], others: dict[str, tuple[int, int]], same: tuple = ()) -> None:
+    """An output overlaps none of the others; those named in `same` it may be as a whole."""
+    a, b = span
+    for other, (c, d) in others.items():
+        if a < d and c < b and not (other in same and a == c):
             raise ValueError(f"{name} must not overlap {other}" + (" unless it is the same tensor" if other in same
                                                                     else ""))
 
 
 def _forward(x, counts, w_in, w_out, act, out, stream, train):
-    m = _checked(x, counts, w_in, w_out, act)
+    m, spans = _checked(x, counts, w_in, w_out, act)
     if out is not None:
-        _rows(out, "out", tuple(x.shape), x)
-        _apart(out, "out", {"x": x, "counts": counts, "w_in": w_in, "w_out": w_out}, () if train else ("x",))
+        _apart("out", _rows(out, "out", x.shape, x), spans, () if train else ("x",))
     with _On(x.device, stream) as s:
-        word = _status_word(x.device)
-        y = torch.empty_like(x) if out is None else out
-        h = torch.empty(m.rows, m.inner, dtype=x.dtype, device=x.device)
-        gu = torch.empty(m.rows, 2, m.inner, dtype=torch.float32, device=x.device) if train else None
-        m.status = word.data_ptr()
+        m.status = _status_word(x.device).data_ptr()
+        y = x.new_empty(x.shape) if out is None else out
+        h = x.new_empty((m.rows, m.inner))
+        gu = x.new_empty((m.rows, 2, m.inner), dtype=torch.float32) if train else None
         check(_lib().ugdr_x_expert_ffn(C.byref(m), x.data_ptr(), y.data_ptr(), h.data_ptr(),
                                        gu.data_ptr() if train else None, s), "ugdr_x_expert_ffn")
     return y, ExpertFFNSaved(h, gu) if train else None
@@ -204,25 +204,22 @@ def expert_ffn_backward(dy: torch.Tensor, x: torch.Tensor, counts: torch.Tensor,
     """(dx, dw_in, dw_out) from dy = d loss / d y and the forward pass's inputs, into the tensors
     given for them.  dx may be dy or x itself.  Weight gradients of experts without rows are
     zeros."""
-    m = _checked(x, counts, w_in, w_out, act)
-    _rows(dy, "dy", tuple(x.shape), x)
-    _rows(saved.h, "saved.h", (m.rows, m.inner), x)
-    _rows(saved.gu, "saved.gu", (m.rows, 2, m.inner), x, torch.float32)
-    inputs = {"dy": dy, "x": x, "counts": counts, "w_in": w_in, "w_out": w_out, "saved.h": saved.h,
-              "saved.gu": saved.gu}
+    m, spans = _checked(x, counts, w_in, w_out, act)
+    spans["dy"] = _rows(dy, "dy", x.shape, x)
+    spans["saved.h"] = _rows(saved.h, "saved.h", (m.rows, m.inner), x)
+    spans["saved.gu"] = _rows(saved.gu, "saved.gu", (m.rows, 2, m.inner), x, torch.float32)
     for name, t, like in (("dx", dx, x), ("dw_in", dw_in, w_in), ("dw_out", dw_out, w_out)):
         if t is not None:
-            _rows(t, name, tuple(like.shape), x)
-            _apart(t, name, inputs, ("dy", "x") if name == "dx" else ())
-            inputs[name] = t
+            span = _rows(t, name, like.shape, x)
+            _apart(name, span, spans, ("dy", "x") if name == "dx" else ())
+            spans[name] = span
     with _On(x.device, stream) as s:
-        word = _status_word(x.device)
-        dx = torch.empty_like(x) if dx is None else dx
-        dw_in = torch.empty_like(w_in) if dw_in is None else dw_in
-        dw_out = torch.empty_like(w_out) if dw_out is None else dw_out
-        dgu = torch.empty(m.rows, 2, m.inner, dtype=x.dtype, device=x.device)
-        m.status = word.data_ptr()
-        check(_lib().ugdr_x_expert_ffn_backward(C.byref(m), dy.data_ptr(), x.data_ptr(), saved.h.data_ptr(),
-                                                saved.gu.data_ptr(), dgu.data_ptr(), dx.data_ptr(),
+        m.status = _status_word(x.device).data_ptr()
+        dx = x.new_empty(x.shape) if dx is None else dx
+        dw_in = x.new_empty(w_in.shape) if dw_in is None else dw_in
+        dw_out = x.new_empty(w_out.shape) if dw_out is None else dw_out
+        dgu = x.new_empty((m.rows, 2, m.inner))
+        check(_lib().ugdr_x_expert_ffn_backward(C.byref(m), spans["dy"][0], spans["x"][0], spans["saved.h"][0],
+                                                spans["saved.gu"][0], dgu.data_ptr(), dx.data_ptr(),
                                                 dw_in.data_ptr(), dw_out.data_ptr(), s), "ugdr_x_expert_ffn_backward")
     return dx, dw_in, dw_out

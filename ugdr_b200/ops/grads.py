@@ -15,7 +15,7 @@ import torch
 
 from .. import _native as N
 from ..parallel.peers import check
-from .experts import _On, _overlap
+from .experts import _On
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 PARTIALS = 2048
@@ -71,7 +71,8 @@ class GradClip:
                 raise ValueError(f"an output of shape {tuple(o.shape)} for a gradient of shape {tuple(g.shape)}")
             if o.dtype not in (g.dtype, torch.float32):
                 raise ValueError(f"an output of {o.dtype} for a gradient of {g.dtype}")
-            if _overlap(g, o) and (o.data_ptr() != g.data_ptr() or o.dtype != g.dtype):
+            apart = o.data_ptr() >= g.data_ptr() + g.nbytes or g.data_ptr() >= o.data_ptr() + o.nbytes
+            if not apart and (o.data_ptr() != g.data_ptr() or o.dtype != g.dtype):
                 raise ValueError("an output must be its gradient or not overlap it")
         self._refuse_overlaps()
         self.device = self.grads[0].device
@@ -108,8 +109,8 @@ class GradClip:
     def sum_squares(self, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
         """The sum of the squares of all elements, a float64 tensor on the device."""
         with _On(self.device, stream) as s:
-            partials = torch.empty(PARTIALS, dtype=torch.float64, device=self.device)
-            total = torch.empty((), dtype=torch.float64, device=self.device)
+            partials = self._plan.new_empty(PARTIALS, dtype=torch.float64)
+            total = self._plan.new_empty((), dtype=torch.float64)
             check(_lib().ugdr_x_grad_sum_squares(self._plan.data_ptr(), self._n, self._chunks, partials.data_ptr(),
                                                  total.data_ptr(), s), "ugdr_x_grad_sum_squares")
         return total
@@ -127,8 +128,8 @@ class GradClip:
                                         or sum_squares.dtype != torch.float64 or sum_squares.device != self.device):
             raise ValueError(f"sum_squares must be one float64 on {self.device}")
         with _On(self.device, stream) as s:
-            partials = torch.empty(PARTIALS, dtype=torch.float64, device=self.device)
-            norm = torch.empty((), dtype=torch.float32, device=self.device)
+            partials = self._plan.new_empty(PARTIALS, dtype=torch.float64)
+            norm = self._plan.new_empty((), dtype=torch.float32)
             check(_lib().ugdr_x_grad_clip(self._plan.data_ptr(), self._n, self._chunks, partials.data_ptr(),
                                           None if sum_squares is None else sum_squares.data_ptr(), max_norm,
                                           norm.data_ptr(), s), "ugdr_x_grad_clip")
