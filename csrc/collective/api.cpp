@@ -1,5 +1,6 @@
 // C ABI of the collective kernels and the IPC helpers that build a peer set.
 #include "collective/kernels.hpp"
+#include "collective/operators.hpp"
 #include "ugdr/collective.h"
 
 #include <cuda.h>
@@ -7,6 +8,7 @@
 
 #include <atomic>
 #include <cstring>
+#include <initializer_list>
 
 namespace {
 
@@ -27,7 +29,7 @@ int default_ctas() {
 using GetRangeFn = CUresult (*)(CUdeviceptr *, size_t *, CUdeviceptr);
 
 // Fills `out` for one kernel: resources from cudaFuncGetAttributes, residency from the
-// occupancy calculator at the kernel's launch block size.
+// occupancy calculator at the kernel's launch block size and dynamic shared memory.
 template <typename Ref> int fill_kernel_attr(const Ref &k, ugdr_x_kernel_attr *out) {
     cudaFuncAttributes a{};
     if (cudaError_t e = cudaFuncGetAttributes(&a, k.fn); e != cudaSuccess) {
@@ -35,7 +37,15 @@ template <typename Ref> int fill_kernel_attr(const Ref &k, ugdr_x_kernel_attr *o
         return int(e);
     }
     int blocks = 0;
-    if (cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, k.fn, k.threads, 0); e != cudaSuccess) {
+    if (k.dynamic_smem > 0) {
+        if (cudaError_t e = cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.dynamic_smem);
+            e != cudaSuccess) {
+            (void)cudaGetLastError();
+            return int(e);
+        }
+    }
+    if (cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, k.fn, k.threads, size_t(k.dynamic_smem));
+        e != cudaSuccess) {
         (void)cudaGetLastError();
         return int(e);
     }
@@ -55,11 +65,14 @@ template <typename Ref> int fill_kernel_attr(const Ref &k, ugdr_x_kernel_attr *o
 extern "C" {
 
 int ugdr_x_collective_kernel_attributes(int index, ugdr_x_kernel_attr *out) {
-    const ugdr::coll::KernelRef *refs = nullptr;
-    const int n = ugdr::coll::collective_kernels(&refs);
     if (out == nullptr || index < 0) return int(cudaErrorInvalidValue);
-    if (index >= n) return -1;
-    return fill_kernel_attr(refs[index], out);
+    for (const auto list : {&ugdr::coll::collective_kernels, &ugdr::coll::expert_kernels, &ugdr::coll::grad_kernels}) {
+        const ugdr::coll::KernelRef *refs = nullptr;
+        const int n = list(&refs);
+        if (index < n) return fill_kernel_attr(refs[index], out);
+        index -= n;
+    }
+    return -1;
 }
 
 uint64_t ugdr_x_set_collective_wait_ns(uint64_t ns) {

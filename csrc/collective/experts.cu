@@ -1063,7 +1063,22 @@ int backward(const ugdr_x_experts &m, const void *dy, const void *x, const void 
     return int(e);
 }
 
+#define UGDR_EXPERT(KERNEL, T, NAME, P, LABEL) \
+    {#KERNEL "<" NAME ", " LABEL ">", reinterpret_cast<const void *>(&KERNEL<T, P>), kThreads, int(shared_bytes(UGDR_X_EXPERTS_MAX))}
+#define UGDR_EXPERT_ROWS(KERNEL, T, NAME)                                                        \
+    UGDR_EXPERT(KERNEL, T, NAME, kUp, "up"), UGDR_EXPERT(KERNEL, T, NAME, kDown, "down"),        \
+        UGDR_EXPERT(KERNEL, T, NAME, kBack, "back"), UGDR_EXPERT(KERNEL, T, NAME, kInput, "input")
+#define UGDR_EXPERT_TYPE(T, NAME)                                                                            \
+    UGDR_EXPERT_ROWS(expert_kernel, T, NAME), UGDR_EXPERT(expert_kernel, T, NAME, kGradOut, "grad out"),     \
+        UGDR_EXPERT(expert_kernel, T, NAME, kGradIn, "grad in"), UGDR_EXPERT_ROWS(expert_split_kernel, T, NAME)
+
 }  // namespace
+
+int expert_kernels(const KernelRef **out) {
+    static const KernelRef refs[] = {UGDR_EXPERT_TYPE(__nv_bfloat16, "bf16"), UGDR_EXPERT_TYPE(__half, "fp16")};
+    *out = refs;
+    return int(sizeof(refs) / sizeof(refs[0]));
+}
 
 int launch_expert_ffn(const ugdr_x_experts &m, const void *x, void *y, void *h, float *gu, cudaStream_t s) {
     return m.type == UGDR_X_TYPE_BF16 ? forward<__nv_bfloat16>(m, x, y, h, gu, s) : forward<__half>(m, x, y, h, gu, s);

@@ -328,6 +328,16 @@ int blocks_for(uint64_t chunks) {
 
 }  // namespace
 
+int grad_kernels(const KernelRef **out) {
+    static const KernelRef refs[] = {
+        {"grad_norm_kernel", reinterpret_cast<const void *>(&grad_norm_kernel), kThreads},
+        {"grad_sum_kernel", reinterpret_cast<const void *>(&grad_sum_kernel), kThreads},
+        {"grad_scale_kernel", reinterpret_cast<const void *>(&grad_scale_kernel), kThreads},
+    };
+    *out = refs;
+    return int(sizeof(refs) / sizeof(refs[0]));
+}
+
 int launch_grad_sum_squares(const void *plan, int n, uint64_t chunks, double *partials, double *sum_squares,
                             cudaStream_t s) {
     const int blocks = blocks_for(chunks);

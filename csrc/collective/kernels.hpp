@@ -32,6 +32,7 @@ struct KernelRef {
     const char *name;
     const void *fn;
     int threads;
+    int dynamic_smem = 0;
 };
 int collective_kernels(const KernelRef **out);
 int launch_allreduce_bf16(const PeerSet &ps, uint64_t offset, uint64_t count, uint64_t epoch, int ctas,

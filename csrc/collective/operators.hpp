@@ -1,6 +1,7 @@
 // Host launch interface of the model operators (experts.cu, grad_clip.cu).
 #pragma once
 
+#include "collective/kernels.hpp"
 #include "ugdr/experts.h"
 
 #include <cuda_runtime_api.h>
@@ -19,5 +20,9 @@ int launch_grad_sum_squares(const void *plan, int n, uint64_t chunks, double *pa
                             cudaStream_t s);
 int launch_grad_clip(const void *plan, int n, uint64_t chunks, double *partials, const double *sum_squares,
                      float max_norm, float *norm_out, cudaStream_t s);
+
+// The operators' kernels, for resource reports.
+int expert_kernels(const KernelRef **out);
+int grad_kernels(const KernelRef **out);
 
 }  // namespace ugdr::coll

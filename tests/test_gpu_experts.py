@@ -347,6 +347,17 @@ def test_refusals():
         ops.expert_ffn_backward(dy[:4], x, c, w_in, w_out, saved)
 
 
+def test_kernel_reports_name_the_operators():
+    from ugdr_b200 import ops
+
+    names = [a["name"] for a in ops.kernel_attributes()]
+    for want in ("expert_kernel<bf16, up>", "expert_kernel<fp16, grad in>", "expert_split_kernel<bf16, down>",
+                 "grad_norm_kernel", "grad_scale_kernel"):
+        assert want in names, names
+    assert all(a["local_bytes_per_thread"] == 0 and a["blocks_per_sm"] == 1 for a in ops.kernel_attributes()
+               if a["name"].startswith("expert"))
+
+
 def test_moe_layer_trains_through_the_exchange():
     """A rank's MoE layer with real experts, as a training step runs it: dispatch, experts, combine,
     the gradients back the same way, the weights' gradients clipped; against fp64.  One expert per
@@ -368,11 +379,13 @@ def test_moe_layer_trains_through_the_exchange():
     counts = moe.expert_rows()
     rows = moe.recv_view().clone()
     _, saved = ops.expert_ffn_train(rows, counts, w_in, w_out, out=moe.recv_view())
+    moe.ready()
     out = moe.combine(w)
     dyt = (dout.float() * w).to(torch.bfloat16)
     moe.dispatch(dyt, ids)
     dx, dw_in, dw_out = ops.expert_ffn_backward(moe.recv_view(), rows, counts, w_in, w_out, saved,
                                                 dx=moe.recv_view())
+    moe.ready()
     dxt = moe.combine(torch.ones_like(w))
     torch.cuda.synchronize()
     g.check_status()
@@ -401,4 +414,5 @@ def test_moe_layer_trains_through_the_exchange():
     # Serving: the experts in place in the receive area.
     moe.dispatch(x, ids)
     ops.expert_ffn(moe.recv_view(), moe.expert_rows(), w_in, w_out, out=moe.recv_view())
+    moe.ready()
     assert torch.equal(moe.combine(w), out)

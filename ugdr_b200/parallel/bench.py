@@ -12,7 +12,8 @@
 * moe: 16,384 tokens x 7,168 bf16 per rank, top-8 of 256 experts from uniform router logits;
   one step = dispatch + combine (experts are the identity).  ugdr fuses the permutes into the
   NVLink stores / loads; the NCCL baseline is all_to_all_single with the permutes as separate
-  torch kernels and the split sizes exchanged first.
+  torch kernels and the split sizes exchanged first.  With --inner F the step is also timed with
+  real experts, gated feed-forward blocks of inner size F, between dispatch and combine.
 Times are CUDA-event durations of K back-to-back iterations on each rank, max over ranks.  The
 first ugdr call is checked against a torch fp32 reference.
 """
@@ -248,7 +249,33 @@ def bench_p2p_nccl(rank, world, sizes, iters, warmup) -> list[dict]:
     return out
 
 
-def bench_moe(rank, world, iters, warmup, cfg: MoEConfig) -> dict:
+def _moe_experts(rank, world, iters, warmup, cfg: MoEConfig, inner, g, a2a, x, ids, w) -> dict:
+    """dispatch, this rank's experts in place in the receive area, combine."""
+    from .. import ops
+
+    T, H, K = cfg.tokens, cfg.hidden, cfg.topk
+    mine = cfg.experts // world
+    gen = torch.Generator(device="cuda").manual_seed(3000 + rank)
+    w_in = torch.empty(mine, 2, inner, H, dtype=x.dtype, device="cuda").normal_(0, H ** -0.5, generator=gen)
+    w_out = torch.empty(mine, H, inner, dtype=x.dtype, device="cuda").normal_(0, inner ** -0.5, generator=gen)
+
+    def step():
+        a2a.dispatch(x, ids)
+        rows = a2a.recv_view()
+        ops.expert_ffn(rows, a2a.expert_rows(), w_in, w_out, out=rows)
+        a2a.ready()
+        return a2a.combine(w)
+
+    t = _timed(step, iters, warmup)
+    g.check_status()
+    ops.check_status()
+    rows = torch.tensor([float(a2a.recv_used.item())], dtype=torch.float64)
+    dist.all_reduce(rows, group=_GLOO)
+    return {"inner": inner, "ugdr_with_experts_ms": round(t, 4),
+            "experts_TFLOPs_per_gpu": round(6 * float(rows) * H * inner / world / t / 1e9, 1)}
+
+
+def bench_moe(rank, world, iters, warmup, cfg: MoEConfig, inner: int = 0) -> dict:
     T, H, K, E = cfg.tokens, cfg.hidden, cfg.topk, cfg.experts
 
     def exchange(obj):
@@ -274,6 +301,8 @@ def bench_moe(rank, world, iters, warmup, cfg: MoEConfig) -> dict:
     ok = torch.allclose(out.float(), ref, atol=3e-2, rtol=2e-2)
     t_ugdr = _timed(ugdr_step, iters, warmup)
     g.check_status()
+
+    experts = _moe_experts(rank, world, iters, warmup, cfg, inner, g, a2a, x, ids, w) if inner else {}
 
     # NCCL baseline: permute by destination rank, exchange split sizes, all_to_all_single,
     # (identity experts), reverse all_to_all_single, weighted un-permute.
@@ -304,7 +333,7 @@ def bench_moe(rank, world, iters, warmup, cfg: MoEConfig) -> dict:
     return {"op": "moe_dispatch_combine", "n_gpus": world, "tokens": T, "hidden": H, "topk": K, "experts": E,
             "ugdr_ms": round(t_ugdr, 4), "nccl_ms": round(t_nccl, 4),
             "ugdr_GBps_per_rank": round(moved / t_ugdr / 1e6, 1), "nccl_GBps_per_rank": round(moved / t_nccl / 1e6, 1),
-            "speedup_vs_nccl": round(t_nccl / t_ugdr, 3), "correct": bool(ok)}
+            "speedup_vs_nccl": round(t_nccl / t_ugdr, 3), "correct": bool(ok), **experts}
 
 
 def bench_moe_verbs(rank, world, local, iters, warmup, cfg: MoEConfig) -> dict:
@@ -389,6 +418,7 @@ def main():
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--ar-mib", type=int, default=1024, help="allreduce bytes per rank, MiB")
     ap.add_argument("--tokens", type=int, default=MoEConfig().tokens, help="MoE tokens per rank")
+    ap.add_argument("--inner", type=int, default=0, help="MoE: also time the step with experts of this inner size")
     ap.add_argument("--ar-impl", default="all", choices=["all", "ring", "nvls"],
                     help="allreduce paths to time (all: ring, NVLS when available, and NCCL)")
     ap.add_argument("--ctas", type=int, default=0, help="allreduce grid size (0: one CTA per SM)")
@@ -424,7 +454,8 @@ def main():
         results.extend(bench_p2p_nccl(rank, world, sizes, max(args.iters, 20), args.warmup))
     if args.op in ("all", "moe"):
         if args.api in ("peer", "both"):
-            results.append(bench_moe(rank, world, args.iters, args.warmup, MoEConfig(tokens=args.tokens)))
+            results.append(bench_moe(rank, world, args.iters, args.warmup, MoEConfig(tokens=args.tokens),
+                                     args.inner))
         if args.api in ("verbs", "both"):
             results.append(bench_moe_verbs(rank, world, local, args.iters, args.warmup, MoEConfig(tokens=args.tokens)))
     if rank == 0:

@@ -40,7 +40,9 @@ class MoEAllToAll:
     [count table: world * nexp int32 | receive area: recv_rows rows of `hidden` bf16].
 
     dispatch(x, ids) sends every (token, k) row to the owner of expert ids[t, k], stored grouped
-    by expert; combine(w) pulls them back and returns sum_k w[t, k] * row(t, k)."""
+    by expert; combine(w) pulls them back and returns sum_k w[t, k] * row(t, k).  In between, the
+    experts work on recv_view() in place (ugdr_b200.ops.expert_ffn with expert_rows()), followed by
+    ready()."""
 
     def __init__(self, group: PeerGroup, tokens: int, hidden: int, topk: int, nexp: int,
                  recv_rows: int):
@@ -95,6 +97,12 @@ class MoEAllToAll:
                                     C.c_void_p(self.ids.data_ptr()), C.c_void_p(self.pos.data_ptr()),
                                     C.c_void_p(self.gbase.data_ptr()), self.tokens, self.topk, self.exp_per_rank,
                                     self.recv_off, self.recv_rows, ep, ctas, s), "ugdr_x_moe_dispatch")
+
+    def ready(self, stream: torch.cuda.Stream | None = None) -> None:
+        """Wait on the device until every rank got here: a combine behind it finds what the experts
+        of all ranks wrote over their receive areas.  (A combine without experts in between needs
+        none: the dispatch ends with every rank's rows in place.)"""
+        allreduce_bf16(self.g, 0, ctas=1, stream=stream)
 
     def combine(self, weights: torch.Tensor, out: torch.Tensor | None = None, ctas: int = 0,
                 stream: torch.cuda.Stream | None = None) -> torch.Tensor:
