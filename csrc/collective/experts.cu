@@ -380,13 +380,14 @@ __device__ __forceinline__ void add8(const float *p, float (&v)[8]) {
     for (int j = 0; j < 8; ++j) v[j] += w[j];
 }
 
-// a(g) and a'(g).  The reciprocal is the approximate one (1 ulp): 1 + exp(-g) is between 1 and
-// infinity, whose reciprocal is the 0 that belongs there.
+// a(g) and a'(g).  silu's exponential and quotient are the approximate ones: together off by less
+// than (|g| + 8) 2^-23 of the value, which goes under in the rounding to 16 bits (2^-12 of it at best).
+// 1 + exp(-g) is between 1 and infinity, whose quotient is the 0 that belongs there.
 struct Act {
     float a, da;
 };
 __device__ __forceinline__ Act silu(float g) {
-    const float s = __fdividef(1.f, 1.f + expf(-g));
+    const float s = __fdividef(1.f, 1.f + __expf(-g));
     return {g * s, s * (1.f + g * (1.f - s))};
 }
 __device__ __forceinline__ Act gelu(float g) {
@@ -699,6 +700,35 @@ template <typename T, Product P> __device__ __forceinline__ Issuer<T, P> issuer_
             {k.stage0, 0, 0}};
 }
 
+// The warp that clears tails: rows behind a group in its last step, up to the next 16, become zeros.
+struct TailClearer {
+    const Shape &m;
+    Shared &sh;
+    const Setup &k;
+    uint32_t it = 0, phases = 0;  // steps so far, and the phase of each stage's barrier for tails
+
+    // After steps [k0, k1) of a tile of a group of `rows`.
+    __device__ __forceinline__ bool clear(int rows, int k0, int k1) {
+        const int last = rows % kDepth;
+        it += uint32_t(k1 - k0);
+        if (k1 == k0 || last == 0 || k1 * kDepth < rows) return true;
+        const uint32_t s = (it - 1) % uint32_t(m.stages);
+        if (!mbar_wait(smem_addr(&sh.tail[s]), phases >> s & 1, sh, m.status)) return false;
+        phases ^= 1u << s;
+        uint8_t *stage = k.ring + s * m.stage_bytes;
+        const int count = ceil_div(last, 16) * 16 - last;  // rows of 128 bytes, in each of 4 tiles
+        for (int i = threadIdx.x % 32; i < count * 4 * 8; i += 32) {
+            const int tile = i / (count * 8), piece = i % (count * 8);
+            reinterpret_cast<uint4 *>(stage + tile * (kDepth * 128) + last * 128)[piece] = make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (threadIdx.x % 32 == 0) mbar_arrive_cluster(map_to(smem_addr(&sh.full[s]), k.leader));
+        __syncwarp();
+        return true;
+    }
+};
+
 // One product, a pair of CTAs per tile.
 template <typename T, Product P>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -727,26 +757,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             ++acc;
         }
     } else if (warp == 2 && kWeightGrad<P>) {
-        // Tails: the rows behind the group in its last step, up to the next 16, become zeros.
-        uint32_t it = 0, phases = 0;
-        for (int at = pair; tiles.next(at, t); at += pairs) {
-            const int last = t.rows % kDepth;
-            it += uint32_t(steps_of<P>(m, t.rows));
-            if (last == 0) continue;
-            const uint32_t s = (it - 1) % uint32_t(m.stages);
-            if (!mbar_wait(smem_addr(&sh.tail[s]), phases >> s & 1, sh, m.status)) break;
-            phases ^= 1u << s;
-            uint8_t *stage = k.ring + s * m.stage_bytes;
-            const int clear = ceil_div(last, 16) * 16 - last;  // rows of 128 bytes, in each of 4 tiles
-            for (int i = lane; i < clear * 4 * 8; i += 32) {
-                const int tile = i / (clear * 8), piece = i % (clear * 8);
-                reinterpret_cast<uint4 *>(stage + tile * (kDepth * 128) + last * 128)[piece] = make_uint4(0, 0, 0, 0);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(map_to(smem_addr(&sh.full[s]), k.leader));
-            __syncwarp();
-        }
+        TailClearer clearer{m, sh, k};
+        for (int at = pair; tiles.next(at, t); at += pairs)
+            if (!clearer.clear(t.rows, 0, steps_of<P>(m, t.rows))) break;
     } else if (warp >= 4) {
         // Finished accumulators.  This warp's TMEM lanes are features 32 (warp % 4) ... + 31; its
         // group of four warps takes every other chunk of columns.
@@ -830,7 +843,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // One product of few tiles: the pairs of a cluster share a tile, each with a part of the steps, and
 // add their sums up through distributed shared memory, in the pairs' order.  A tile's K loop runs at
 // the latency of its ring, so one pair reads weights at a few hundred GB/s however idle the GPU is:
-// a [1, 5632] x [5632, 2048] product has 8 tiles, and took 26 us with a pair each.
+// a [1, 5632] x [5632, 2048] product has 8 tiles, and took 26 us with a pair each.  Likewise a weight
+// gradient over 25,000 rows of one expert with 10 tiles: 120 us.
 template <typename T, Product P>
 __global__ void __launch_bounds__(kThreads, 1)
     expert_split_kernel(const __grid_constant__ Maps maps, const Shape m, T *out, float *gu) {
@@ -839,30 +853,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int split = int(cluster_size()) / 2, part = int(k.leader) / 2;
     const int cluster = int(blockIdx.x) / (2 * split), clusters = int(gridDim.x) / (2 * split);
-    const int steps = steps_of<P>(m, 0), k0 = steps * part / split, k1 = steps * (part + 1) / split;
     Tiles<P> tiles(m, k.first);
     Tile t;
     Loader<P> loader = loader_of<P>(maps, m, k);
     Issuer<T, P> issuer = issuer_of<T, P>(m, k);
+    TailClearer clearer{m, sh, k};
     float *sums = reinterpret_cast<float *>(k.ring);  // [part][column][feature], once the ring is idle
     uint32_t phase = 0;
 
     for (int at = cluster; tiles.next(at, t); at += clusters) {
-        const int n = ceil_div(t.rows, kStepN) * kStepN, columns = n / split;  // columns that each pair adds up
+        const int steps = steps_of<P>(m, t.rows), k0 = steps * part / split, k1 = steps * (part + 1) / split;
+        const int n = kWeightGrad<P> ? kMaxN : ceil_div(t.rows, kStepN) * kStepN, columns = n / split;  // each pair's
         const int feature = t.feature + int(k.rank) * (kTileFeatures<P> / 2);
         if (warp == 0 && lane == 0) {
             loader.load_tile(t, k0, k1);
         } else if (warp == 1 && lane == 0 && k.rank == 0) {
-            if (issuer.run(t, sh.tmem, k0, k1)) mma_commit(smem_addr(&sh.tmem_full[0]), issuer.mask);
-        } else if (warp >= 4) {
+            if (k1 > k0 && issuer.run(t, sh.tmem, k0, k1)) mma_commit(smem_addr(&sh.tmem_full[0]), issuer.mask);
+        } else if (warp == 2 && kWeightGrad<P>) {
+            clearer.clear(t.rows, k0, k1);
+        } else if (warp >= 4 && k1 > k0) {
             mbar_wait(smem_addr(&sh.tmem_full[0]), phase, sh, m.status);
         }
-        phase ^= 1;
+        phase ^= uint32_t(k1 > k0);
         __syncthreads();
         const bool fine = !sh.aborted;
         cluster_sync();  // every pair's products are over, and no load is under way
         fence_after();
-        if (fine && warp >= 4) {
+        if (fine && warp >= 4 && k1 > k0) {
             const int quarter = warp % 4, group = warp / 4 - 1;
             for (int c = group * 8; c < n; c += 16) {
                 float v[8];
@@ -875,10 +892,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         fence_before();
         cluster_sync();  // the sums are there
-        const int mine = min(columns, t.rows - part * columns);
-        if (fine) {
+        if constexpr (kWeightGrad<P>) {
+            // A thread adds up 8 columns of one row of the gradient.
+            const int width = P == kGradOut ? m.inner : m.hidden, height = P == kGradOut ? m.hidden : m.inner;
+            for (int i = threadIdx.x; fine && i < kHalf * (columns / 8); i += kThreads) {
+                const int f = feature + i % kHalf, c = i / kHalf * 8, column = t.column + part * columns + c;
+                if (f >= height || column >= width) continue;
+                float a[8] = {};
+                for (int p = 0; p < split; ++p) {
+                    if (steps * p / split == steps * (p + 1) / split) continue;  // had no steps
+                    const float *from = sums + (p * columns + c) * kStagingRow + i % kHalf;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) a[j] += from[j * kStagingRow];
+                }
+                store8(out + ((int64_t(t.expert) * (P == kGradIn ? 2 : 1) + t.part) * height + f) * width + column, a);
+            }
+        } else {
             constexpr int kGroups = P == kUp ? 8 : 16;
-            for (int i = threadIdx.x; i < mine * kGroups; i += kThreads) {
+            const int mine = min(columns, t.rows - part * columns);
+            for (int i = threadIdx.x; fine && i < mine * kGroups; i += kThreads) {
                 const int column = i / kGroups, f = feature + i % kGroups * 8;
                 const int64_t row = t.first + part * columns + column;
                 if (f >= (P == kUp || P == kBack ? m.inner : m.hidden)) continue;
@@ -963,13 +995,19 @@ cudaError_t prepare(const void *kernel, int device, int index, int *sms) {
 
 // Pairs that share a tile: as many as keep every tile's pairs on the GPU at once, with four steps or
 // more for each.  What counts is known here from above only: a tile for each expert, or row if those
-// are fewer, and one for every kMaxN rows.
+// are fewer, and one for every kMaxN rows; for the weight gradients, whose steps are an expert's
+// rows, their mean.
 template <Product P> int split_of(const ugdr_x_experts &m, int pairs) {
-    if (kWeightGrad<P>) return 1;
-    const int64_t row_tiles = (m.rows < uint64_t(m.nexp) ? int64_t(m.rows) : m.nexp) + int64_t(m.rows / kMaxN);
-    const int64_t features = P == kUp || P == kBack ? m.inner : m.hidden;
-    const int64_t tiles = row_tiles * ((features + kTileFeatures<P> - 1) / kTileFeatures<P>);
-    const int64_t depth = P == kDown ? m.inner : P == kInput ? 2 * int64_t(m.inner) : m.hidden;
+    const auto tiles_of = [](int64_t n, int64_t size) { return (n + size - 1) / size; };
+    const int64_t features = P == kUp || P == kBack || P == kGradIn ? m.inner : m.hidden;
+    int64_t tiles = tiles_of(features, kTileFeatures<P>), depth = 0;
+    if (kWeightGrad<P>) {
+        tiles *= m.nexp * (P == kGradIn ? 2 : 1) * tiles_of(P == kGradOut ? m.inner : m.hidden, kMaxN);
+        depth = int64_t(m.rows / uint64_t(m.nexp));
+    } else {
+        tiles *= (m.rows < uint64_t(m.nexp) ? int64_t(m.rows) : m.nexp) + int64_t(m.rows / kMaxN);
+        depth = P == kDown ? m.inner : P == kInput ? 2 * int64_t(m.inner) : m.hidden;
+    }
     for (int split = kMaxSplit; split > 1; split /= 2)
         if (tiles * split <= pairs && depth >= 4 * split * kDepth) return split;
     return 1;
@@ -1029,18 +1067,14 @@ cudaError_t launch(const ugdr_x_experts &m, const void *a, const void *b, void *
     config.stream = s;
     config.attrs = attributes;
     config.numAttrs = 1;
-    if constexpr (!kWeightGrad<P>) {
-        const int split = split_of<P>(m, sms / 2);
-        if (split > 1) {
-            kernel = expert_split_kernel<T, P>;
-            if (cudaError_t e = prepare(reinterpret_cast<const void *>(kernel), device, 12 + kIndex, &sms);
-                e != cudaSuccess)
-                return e;
-            attributes[1].id = cudaLaunchAttributeClusterDimension;
-            attributes[1].val.clusterDim = {unsigned(2 * split), 1, 1};
-            config.gridDim = dim3(unsigned(sms / (2 * split) * (2 * split)));
-            config.numAttrs = 2;
-        }
+    if (const int split = split_of<P>(m, sms / 2); split > 1) {
+        kernel = expert_split_kernel<T, P>;
+        if (cudaError_t e = prepare(reinterpret_cast<const void *>(kernel), device, 12 + kIndex, &sms); e != cudaSuccess)
+            return e;
+        attributes[1].id = cudaLaunchAttributeClusterDimension;
+        attributes[1].val.clusterDim = {unsigned(2 * split), 1, 1};
+        config.gridDim = dim3(unsigned(sms / (2 * split) * (2 * split)));
+        config.numAttrs = 2;
     }
     return cudaLaunchKernelEx(&config, kernel, maps, shape, static_cast<T *>(out), gu);
 }
@@ -1065,17 +1099,17 @@ int backward(const ugdr_x_experts &m, const void *dy, const void *x, const void 
 
 #define UGDR_EXPERT(KERNEL, T, NAME, P, LABEL) \
     {#KERNEL "<" NAME ", " LABEL ">", reinterpret_cast<const void *>(&KERNEL<T, P>), kThreads, int(shared_bytes(UGDR_X_EXPERTS_MAX))}
-#define UGDR_EXPERT_ROWS(KERNEL, T, NAME)                                                        \
-    UGDR_EXPERT(KERNEL, T, NAME, kUp, "up"), UGDR_EXPERT(KERNEL, T, NAME, kDown, "down"),        \
-        UGDR_EXPERT(KERNEL, T, NAME, kBack, "back"), UGDR_EXPERT(KERNEL, T, NAME, kInput, "input")
-#define UGDR_EXPERT_TYPE(T, NAME)                                                                            \
-    UGDR_EXPERT_ROWS(expert_kernel, T, NAME), UGDR_EXPERT(expert_kernel, T, NAME, kGradOut, "grad out"),     \
-        UGDR_EXPERT(expert_kernel, T, NAME, kGradIn, "grad in"), UGDR_EXPERT_ROWS(expert_split_kernel, T, NAME)
+#define UGDR_EXPERT_ALL(KERNEL, T, NAME)                                                                    \
+    UGDR_EXPERT(KERNEL, T, NAME, kUp, "up"), UGDR_EXPERT(KERNEL, T, NAME, kDown, "down"),                    \
+        UGDR_EXPERT(KERNEL, T, NAME, kBack, "back"), UGDR_EXPERT(KERNEL, T, NAME, kInput, "input"),          \
+        UGDR_EXPERT(KERNEL, T, NAME, kGradOut, "grad out"), UGDR_EXPERT(KERNEL, T, NAME, kGradIn, "grad in")
 
 }  // namespace
 
 int expert_kernels(const KernelRef **out) {
-    static const KernelRef refs[] = {UGDR_EXPERT_TYPE(__nv_bfloat16, "bf16"), UGDR_EXPERT_TYPE(__half, "fp16")};
+    static const KernelRef refs[] = {
+        UGDR_EXPERT_ALL(expert_kernel, __nv_bfloat16, "bf16"), UGDR_EXPERT_ALL(expert_kernel, __half, "fp16"),
+        UGDR_EXPERT_ALL(expert_split_kernel, __nv_bfloat16, "bf16"), UGDR_EXPERT_ALL(expert_split_kernel, __half, "fp16")};
     *out = refs;
     return int(sizeof(refs) / sizeof(refs[0]));
 }
