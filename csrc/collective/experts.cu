@@ -51,6 +51,7 @@ constexpr int kBoxes = 4;           // TMA boxes of 128, 64, 32 and 16 rows
 constexpr int kMaxStages = 10;
 constexpr int kMaxSplit = 4;
 constexpr int kChunk = 16;          // rows (or columns of a gradient) that an epilogue group moves at once
+constexpr int kMaxOrdered = 512;
 constexpr int kBand = 8;            // row tiles that run through all features before the next
 constexpr uint32_t kOperandBytes = kHalf * kDepth * 2;  // one CTA's half of A, or of B for the largest N
 constexpr uint32_t kRingBytes = 6 * 2 * kOperandBytes;  // 6 stages for the largest N, 10 for the smallest
@@ -76,6 +77,7 @@ struct Shared {
     uint32_t tmem;
     int aborted;
     long long scan[kThreads / 32];
+    uint16_t order[kMaxOrdered];  // weight gradients: the experts, those with the most rows first
 };
 constexpr size_t shared_bytes(int nexp) {
     return 1024 + kRingBytes + 2 * kStagingBytes + sizeof(Shared) + (size_t(nexp) + 1) * 4;
@@ -206,17 +208,23 @@ __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.w
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
-// 16 columns of this warp's 32 TMEM lanes: v[j] is column j of lane threadIdx.x % 32.
-__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[kChunk]) {
-    uint32_t *r = reinterpret_cast<uint32_t *>(v);
+// 16 columns of this warp's 32 TMEM lanes: v[j] is column j of lane threadIdx.x % 32, once
+// tmem_wait() is over.
+__device__ __forceinline__ void tmem_request(uint32_t addr, uint32_t (&r)[kChunk]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
-                 "tcgen05.wait::ld.sync.aligned;"
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
                    "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
                    "=r"(r[15])
                  : "r"(addr)
                  : "memory");
+}
+// The registers pass through, so that no use of them can move before the wait.
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[kChunk]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15])::"memory");
 }
 __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[8]) {
     uint32_t *r = reinterpret_cast<uint32_t *>(v);
@@ -261,26 +269,36 @@ template <Product P> __device__ __forceinline__ int steps_of(const Shape &m, int
     return ceil_div(P == kDown ? m.inner : m.hidden, kDepth);
 }
 
-// Walks the tile list in order: next() finds tile t for increasing t.
+// Walks a worker's share of the tile list: one tile of every round.
 //
 // An expert's rows are cut into tiles of about the same size, all but the last a multiple of kStepN.
 // (Tiles of up to 512 rows, in both accumulators, load the features once for more rows; they gained
 // 4 % at 300 rows per expert and cost 1 to 4 % elsewhere, for the longer code and the accumulators
 // that no products run beside.)
+//
+// A weight gradient's tiles take as long as their expert has rows, so the experts with the most rows
+// come first, and the pairs take turns forwards and backwards: 22,539 rows over 23 uneven experts,
+// 784 x 168, took 333 us in the experts' order, and 262 this way.
 template <Product P> struct Tiles {
     const int *first;  // first row of each expert's group, and the end of the last
-    int nexp, mtiles, mparts, ntiles;
-    int expert = -1, base = 0, size = 0, n = 0, columns = 0, per = 0;
+    const uint16_t *order;
+    int nexp, mtiles, mparts, ntiles, worker, workers;
+    int turn = 0, at = -1, expert = 0, base = 0, size = 0, n = 0, columns = 0, per = 0;
 
-    __device__ Tiles(const Shape &m, const int *first_) : first(first_), nexp(m.nexp) {
+    // `worker` of those that share the list.
+    __device__ Tiles(const Shape &m, const int *first_, const uint16_t *order_, int worker_, int workers_)
+        : first(first_), order(order_), nexp(m.nexp), worker(worker_), workers(workers_) {
         const int features = P == kUp || P == kBack || P == kGradIn ? m.inner : m.hidden;
         mparts = ceil_div(features, kTileFeatures<P>);
         mtiles = P == kGradIn ? 2 * mparts : mparts;
         ntiles = P == kGradOut ? ceil_div(m.inner, kMaxN) : P == kGradIn ? ceil_div(m.hidden, kMaxN) : 0;
     }
-    __device__ __forceinline__ bool next(int t, Tile &out) {
+    __device__ __forceinline__ bool next(Tile &out) {
+        const int t = turn * workers + (kWeightGrad<P> && (turn & 1) ? workers - 1 - worker : worker);
+        ++turn;
         while (t >= base + size) {
-            if (++expert >= nexp) return false;
+            if (++at >= nexp) return false;
+            expert = kWeightGrad<P> && nexp <= kMaxOrdered ? order[at] : at;
             base += size;
             n = first[expert + 1] - first[expert];
             columns = kWeightGrad<P> ? ntiles : ceil_div(n, kMaxN);
@@ -350,6 +368,19 @@ __device__ void scan_counts(const Shape &m, Shared &sh, int *first) {
     if (bad && blockIdx.x == 0) atomicExch(m.status, 2u);
 }
 
+// The experts by their rows, the most first, equal ones in their order.
+__device__ void order_experts(const Shape &m, const int *first, uint16_t *order) {
+    for (int e = threadIdx.x; e < m.nexp; e += kThreads) {
+        const int n = first[e + 1] - first[e];
+        int before = 0;
+        for (int o = 0; o < m.nexp; ++o) {
+            const int other = first[o + 1] - first[o];
+            before += other > n || (other == n && o < e);
+        }
+        order[before] = uint16_t(e);
+    }
+}
+
 // ---- elements ----------------------------------------------------------------------------------
 
 __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
@@ -364,9 +395,25 @@ template <typename T> __device__ __forceinline__ void store8(T *p, const float *
     *reinterpret_cast<uint4 *>(p) =
         make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
 }
+// A whole 32-byte sector of global memory at once: halves of one, stored one after the other, are two
+// writes for the L2.
 __device__ __forceinline__ void store8(float *p, const float *v) {
-    reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+                 "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                 : "memory");
+}
+template <typename T> __device__ __forceinline__ void store16(T *p, const float *v) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(pack2(v[0], v[1], T())),
+                 "r"(pack2(v[2], v[3], T())), "r"(pack2(v[4], v[5], T())), "r"(pack2(v[6], v[7], T())),
+                 "r"(pack2(v[8], v[9], T())), "r"(pack2(v[10], v[11], T())), "r"(pack2(v[12], v[13], T())),
+                 "r"(pack2(v[14], v[15], T()))
+                 : "memory");
+}
+__device__ __forceinline__ void load8_global(const float *p, float *v) {
+    asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "l"(p)
+                 : "memory");
 }
 __device__ __forceinline__ void load8(const float *p, float *v) {
     const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
@@ -665,6 +712,10 @@ template <Product P> __device__ __forceinline__ Setup set_up(const Maps &maps, c
     launch_next();  // only now, so that the next kernel of the call finds the call's inputs complete
     scan_counts(m, sh, k.first);
     __syncthreads();
+    if (kWeightGrad<P> && m.nexp <= kMaxOrdered) {
+        order_experts(m, k.first, sh.order);
+        __syncthreads();
+    }
     return k;
 }
 
@@ -736,18 +787,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const Setup k = set_up<P>(maps, m);
     Shared &sh = *k.sh;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, pair = blockIdx.x / 2, pairs = gridDim.x / 2;
-    Tiles<P> tiles(m, k.first);
+    Tiles<P> tiles(m, k.first, sh.order, pair, pairs);
     Tile t;
     uint32_t acc = 0;  // accumulators used so far: they take turns
 
     if (warp == 0 && lane == 0) {
         Loader<P> loader = loader_of<P>(maps, m, k);
-        for (int at = pair; tiles.next(at, t); at += pairs)
+        while (tiles.next(t))
             if (!loader.load_tile(t, 0, steps_of<P>(m, t.rows))) break;
         wait_previous();  // in any case: a kernel is over only when those before it are
     } else if (warp == 1 && lane == 0 && k.rank == 0) {
         Issuer<T, P> issuer = issuer_of<T, P>(m, k);
-        for (int at = pair; tiles.next(at, t); at += pairs) {
+        while (tiles.next(t)) {
             const int steps = steps_of<P>(m, t.rows);
             if (steps == 0) continue;
             if (!mbar_wait(smem_addr(&sh.tmem_empty[acc & 1]), (acc / 2 + 1) & 1, sh, m.status)) break;
@@ -758,14 +809,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 2 && kWeightGrad<P>) {
         TailClearer clearer{m, sh, k};
-        for (int at = pair; tiles.next(at, t); at += pairs)
+        while (tiles.next(t))
             if (!clearer.clear(t.rows, 0, steps_of<P>(m, t.rows))) break;
     } else if (warp >= 4) {
         // Finished accumulators.  This warp's TMEM lanes are features 32 (warp % 4) ... + 31; its
         // group of four warps takes every other chunk of columns.
         const int quarter = warp % 4, group = warp / 4 - 1;
         const uint32_t lanes = sh.tmem + (uint32_t(quarter * 32) << 16), empty = map_to(smem_addr(sh.tmem_empty), k.leader);
-        for (int at = pair; tiles.next(at, t); at += pairs) {
+        while (tiles.next(t)) {
             const bool none = steps_of<P>(m, t.rows) == 0;
             const int feature = t.feature + int(k.rank) * (kTileFeatures<P> / 2);
             if (!none) {
@@ -779,18 +830,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int width = P == kGradOut ? m.inner : m.hidden, height = P == kGradOut ? m.hidden : m.inner;
                 const int f = feature + quarter * 32 + lane;
                 T *row = out + ((int64_t(t.expert) * (P == kGradIn ? 2 : 1) + t.part) * height + f) * width + t.column;
+                const bool sectors = width % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 32 == 0;
+                uint32_t r[kChunk];
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) r[j] = 0;
+                if (!none) tmem_request(columns + group * kChunk, r);
                 for (int c = group * kChunk; c < kMaxN; c += 2 * kChunk) {
                     float v[kChunk];
-                    if (none) {
+                    if (!none) tmem_wait(r);
 #pragma unroll
-                        for (int j = 0; j < kChunk; ++j) v[j] = 0.f;
+                    for (int j = 0; j < kChunk; ++j) v[j] = __uint_as_float(r[j]);
+                    if (!none && c + 2 * kChunk < kMaxN) tmem_request(columns + c + 2 * kChunk, r);
+                    if (f >= height || t.column + c >= width) continue;
+                    if (sectors) {
+                        store16(row + c, v);
                     } else {
-                        tmem_load(columns + c, v);
-                    }
-                    if (f < height) {
-#pragma unroll
-                        for (int j = 0; j < kChunk; j += 8)
-                            if (t.column + c + j < width) store8(row + c + j, v + j);
+                        store8(row + c, v);
+                        if (t.column + c + 8 < width) store8(row + c + 8, v + 8);
                     }
                 }
             } else {
@@ -798,6 +854,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 // of a row's features, 8 next to each other per lane.
                 const int r = quarter * 4 + lane / 8;
                 float *buffer = k.staging + group * (kStagingBytes / 4);
+                uint32_t v[kChunk];
+                if (group * kChunk < t.rows) tmem_request(columns + group * kChunk, v);
                 for (int c = group * kChunk; c < t.rows; c += 2 * kChunk) {
                     const int64_t row = t.first + c + r;
                     float g[2][8], u[2][8];
@@ -806,15 +864,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         for (int i = 0; i < 2; ++i) {
                             const int f = feature + i * 64 + lane % 8 * 8;
                             if (c + r < t.rows && f < m.inner) {
-                                load8(gu + row * 2 * m.inner + f, g[i]);
-                                load8(gu + row * 2 * m.inner + m.inner + f, u[i]);
+                                load8_global(gu + row * 2 * m.inner + f, g[i]);
+                                load8_global(gu + row * 2 * m.inner + m.inner + f, u[i]);
                             }
                         }
                     }
-                    float v[kChunk];
-                    tmem_load(columns + c, v);
+                    tmem_wait(v);
 #pragma unroll
-                    for (int j = 0; j < kChunk; ++j) buffer[j * kStagingRow + quarter * 32 + lane] = v[j];
+                    for (int j = 0; j < kChunk; ++j)
+                        buffer[j * kStagingRow + quarter * 32 + lane] = __uint_as_float(v[j]);
+                    if (c + 2 * kChunk < t.rows) tmem_request(columns + c + 2 * kChunk, v);
                     group_sync(group);
                     const float *sums = buffer + r * kStagingRow + lane % 8 * 8;
 #pragma unroll
@@ -853,7 +912,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int split = int(cluster_size()) / 2, part = int(k.leader) / 2;
     const int cluster = int(blockIdx.x) / (2 * split), clusters = int(gridDim.x) / (2 * split);
-    Tiles<P> tiles(m, k.first);
+    Tiles<P> tiles(m, k.first, sh.order, cluster, clusters);
     Tile t;
     Loader<P> loader = loader_of<P>(maps, m, k);
     Issuer<T, P> issuer = issuer_of<T, P>(m, k);
@@ -861,7 +920,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float *sums = reinterpret_cast<float *>(k.ring);  // [part][column][feature], once the ring is idle
     uint32_t phase = 0;
 
-    for (int at = cluster; tiles.next(at, t); at += clusters) {
+    while (tiles.next(t)) {
         const int steps = steps_of<P>(m, t.rows), k0 = steps * part / split, k1 = steps * (part + 1) / split;
         const int n = kWeightGrad<P> ? kMaxN : ceil_div(t.rows, kStepN) * kStepN, columns = n / split;  // each pair's
         const int feature = t.feature + int(k.rank) * (kTileFeatures<P> / 2);
@@ -916,8 +975,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (f >= (P == kUp || P == kBack ? m.inner : m.hidden)) continue;
                 float a[8] = {}, b[8] = {}, g[8], u[8];
                 if constexpr (P == kBack) {
-                    load8(gu + row * 2 * m.inner + f, g);
-                    load8(gu + row * 2 * m.inner + m.inner + f, u);
+                    load8_global(gu + row * 2 * m.inner + f, g);
+                    load8_global(gu + row * 2 * m.inner + m.inner + f, u);
                 }
                 for (int p = 0; p < split; ++p) {
                     const float *from = sums + (p * columns + column) * kStagingRow + i % kGroups * 8;

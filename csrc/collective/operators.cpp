@@ -6,6 +6,7 @@
 namespace {
 
 bool aligned16(const void *p) { return p != nullptr && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool aligned32(const void *p) { return p != nullptr && reinterpret_cast<uintptr_t>(p) % 32 == 0; }
 
 bool valid(const ugdr_x_experts *m) {
     return m != nullptr && m->counts != nullptr && m->status != nullptr && aligned16(m->w_in) && aligned16(m->w_out) &&
@@ -24,7 +25,7 @@ extern "C" {
 int ugdr_x_expert_ffn(const ugdr_x_experts *m, const void *x, void *y, void *h, float *gu, void *stream) {
     if (!valid(m)) return int(cudaErrorInvalidValue);
     if (m->rows == 0) return int(cudaSuccess);
-    if (!aligned16(x) || !aligned16(y) || !aligned16(h) || (gu != nullptr && !aligned16(gu)))
+    if (!aligned16(x) || !aligned16(y) || !aligned16(h) || (gu != nullptr && !aligned32(gu)))
         return int(cudaErrorInvalidValue);
     return ugdr::coll::launch_expert_ffn(*m, x, y, h, gu, static_cast<cudaStream_t>(stream));
 }
@@ -38,7 +39,7 @@ int ugdr_x_expert_ffn_backward(const ugdr_x_experts *m, const void *dy, const vo
         if (const cudaError_t e = cudaMemsetAsync(dw_in, 0, 2 * block, s); e != cudaSuccess) return int(e);
         return int(cudaMemsetAsync(dw_out, 0, block, s));
     }
-    if (!aligned16(dy) || !aligned16(x) || !aligned16(h) || !aligned16(gu) || !aligned16(dgu) || !aligned16(dx))
+    if (!aligned16(dy) || !aligned16(x) || !aligned16(h) || !aligned32(gu) || !aligned16(dgu) || !aligned16(dx))
         return int(cudaErrorInvalidValue);
     return ugdr::coll::launch_expert_ffn_backward(*m, dy, x, h, gu, dgu, dx, dw_in, dw_out, s);
 }

@@ -45,8 +45,8 @@ typedef struct ugdr_x_experts {
 } ugdr_x_experts;
 
 /* Forward: g = x Wg^T, u = x Wu^T, h = a(g) * u, y = h Wo^T.  `h` ([rows][inner]) is scratch of a
- * serving call; with `gu` ([rows][2][inner] floats, may be NULL) g and u are kept too, and h and gu
- * are what the backward pass takes.  y may be x itself (the products with x are over by then). */
+ * serving call; with `gu` ([rows][2][inner] floats on a 32-byte boundary, may be NULL) g and u are kept
+ * too, and h and gu are what the backward pass takes.  y may be x itself (the products with x are over by then). */
 int ugdr_x_expert_ffn(const ugdr_x_experts *m, const void *x, void *y, void *h, float *gu, void *stream);
 
 /* Backward of y with respect to x and the weights, from dy and what the forward pass kept:

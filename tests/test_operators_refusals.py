@@ -33,7 +33,7 @@ def test_the_block_refuses_what_it_cannot_do(change):
 
 @pytest.mark.parametrize("pointers", [(None, 0x6000, 0x7000, None), (0x5008, 0x6000, 0x7000, None),
                                       (0x5000, None, 0x7000, None), (0x5000, 0x6000, 0x7002, None),
-                                      (0x5000, 0x6000, 0x7000, 0x8001)])
+                                      (0x5000, 0x6000, 0x7000, 0x8001), (0x5000, 0x6000, 0x7000, 0x8010)])
 def test_the_forward_refuses_missing_and_misaligned_tensors(pointers):
     from ugdr_b200.ops.experts import _lib
 

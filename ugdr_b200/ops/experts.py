@@ -208,6 +208,8 @@ def expert_ffn_backward(dy: torch.Tensor, x: torch.Tensor, counts: torch.Tensor,
     spans["dy"] = _rows(dy, "dy", x.shape, x)
     spans["saved.h"] = _rows(saved.h, "saved.h", (m.rows, m.inner), x)
     spans["saved.gu"] = _rows(saved.gu, "saved.gu", (m.rows, 2, m.inner), x, torch.float32)
+    if spans["saved.gu"][0] % 32:
+        raise ValueError("saved.gu must be 32-byte aligned")
     for name, t, like in (("dx", dx, x), ("dw_in", dw_in, w_in), ("dw_out", dw_out, w_out)):
         if t is not None:
             span = _rows(t, name, like.shape, x)
