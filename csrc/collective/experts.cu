@@ -855,25 +855,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int r = quarter * 4 + lane / 8;
                 float *buffer = k.staging + group * (kStagingBytes / 4);
                 uint32_t v[kChunk];
-                if (group * kChunk < t.rows) tmem_request(columns + group * kChunk, v);
-                for (int c = group * kChunk; c < t.rows; c += 2 * kChunk) {
-                    const int64_t row = t.first + c + r;
-                    float g[2][8], u[2][8];
-                    if constexpr (P == kBack) {  // under way while the accumulators are turned around
+                [[maybe_unused]] float g[2][8], u[2][8];  // kBack: the projections of the next chunk's rows
+                const auto request = [&](int c) {
+                    if (c >= t.rows) return;
+                    tmem_request(columns + c, v);
+                    if constexpr (P == kBack) {
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const int f = feature + i * 64 + lane % 8 * 8;
+                            const int64_t row = t.first + c + r;
                             if (c + r < t.rows && f < m.inner) {
                                 load8_global(gu + row * 2 * m.inner + f, g[i]);
                                 load8_global(gu + row * 2 * m.inner + m.inner + f, u[i]);
                             }
                         }
                     }
+                };
+                request(group * kChunk);
+                for (int c = group * kChunk; c < t.rows; c += 2 * kChunk) {
+                    const int64_t row = t.first + c + r;
                     tmem_wait(v);
 #pragma unroll
                     for (int j = 0; j < kChunk; ++j)
                         buffer[j * kStagingRow + quarter * 32 + lane] = __uint_as_float(v[j]);
-                    if (c + 2 * kChunk < t.rows) tmem_request(columns + c + 2 * kChunk, v);
+                    [[maybe_unused]] float gc[2][8], uc[2][8];
+                    if constexpr (P == kBack) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) gc[j / 8][j % 8] = g[j / 8][j % 8], uc[j / 8][j % 8] = u[j / 8][j % 8];
+                    }
+                    request(c + 2 * kChunk);
                     group_sync(group);
                     const float *sums = buffer + r * kStagingRow + lane % 8 * 8;
 #pragma unroll
@@ -883,7 +893,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         float a[8], b[8];
                         load8(sums + i * 64, a);
                         if (P == kUp) load8(sums + 64, b);
-                        finish<T, P>(m, out, gu, row, f, a, b, g[i], u[i]);
+                        finish<T, P>(m, out, gu, row, f, a, b, gc[i], uc[i]);
                     }
                     group_sync(group);  // the buffer is free again
                 }
