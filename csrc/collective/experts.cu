@@ -49,7 +49,6 @@ constexpr int kStepN = 32;
 constexpr int kDepth = 64;          // elements per stage along the summed dimension: 128 bytes
 constexpr int kBoxes = 4;           // TMA boxes of 128, 64, 32 and 16 rows
 constexpr int kMaxStages = 10;
-constexpr int kMaxSplit = 4;
 constexpr int kChunk = 16;          // rows (or columns of a gradient) that an epilogue group moves at once
 constexpr int kMaxOrdered = 512;
 constexpr int kBand = 8;            // row tiles that run through all features before the next
@@ -1043,30 +1042,51 @@ template <typename T> bool encode(CUtensorMap *map, const Dense &d) {
                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Once per kernel and device: its shared memory.  The device's SM count in *sms.
-cudaError_t prepare(const void *kernel, int device, int index, int *sms) {
-    constexpr int kDevices = 64;
-    static std::atomic<int> known_sms[kDevices];
-    static std::atomic<uint32_t> done[kDevices];
+// What a kernel can have on a device at once, asked for once: CTAs (one per SM), or clusters of 4 and
+// 8 CTAs, of which fewer fit than the SMs' number says, since a cluster lies within one GPC.
+struct Residency {
+    int sms, clusters4, clusters8;
+};
+cudaError_t residency(const void *kernel, bool split, int device, int index, Residency *out) {
+    constexpr int kDevices = 64, kKernels = 24;
+    static std::atomic<uint64_t> known[kDevices][kKernels];  // sms, clusters8 and clusters4, 16 bits each
     const bool kept = device < kDevices;
-    *sms = kept ? known_sms[device].load(std::memory_order_relaxed) : 0;
-    if (*sms == 0) {
-        if (cudaError_t e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device); e != cudaSuccess)
-            return e;
-        if (kept) known_sms[device].store(*sms, std::memory_order_relaxed);
+    if (uint64_t v = kept ? known[device][index].load(std::memory_order_acquire) : 0; v != 0) {
+        *out = {int(v & 0xffff), int(v >> 32 & 0xffff), int(v >> 16 & 0xffff)};
+        return cudaSuccess;
     }
-    if (kept && (done[device].load(std::memory_order_relaxed) >> index & 1)) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               int(shared_bytes(UGDR_X_EXPERTS_MAX)));
-    if (e == cudaSuccess && kept) done[device].fetch_or(1u << index, std::memory_order_relaxed);
-    return e;
+    *out = {};
+    constexpr int kBytes = int(shared_bytes(UGDR_X_EXPERTS_MAX));
+    if (cudaError_t e = cudaDeviceGetAttribute(&out->sms, cudaDevAttrMultiProcessorCount, device); e != cudaSuccess)
+        return e;
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+        e != cudaSuccess)
+        return e;
+    for (unsigned size = 4; split && size <= 8; size *= 2) {
+        cudaLaunchAttribute attribute{};
+        attribute.id = cudaLaunchAttributeClusterDimension;
+        attribute.val.clusterDim = {size, 1, 1};
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(size);
+        config.blockDim = dim3(kThreads);
+        config.dynamicSmemBytes = kBytes;
+        config.attrs = &attribute;
+        config.numAttrs = 1;
+        if (cudaError_t e = cudaOccupancyMaxActiveClusters(size == 4 ? &out->clusters4 : &out->clusters8, kernel, &config);
+            e != cudaSuccess)
+            return e;
+    }
+    if (kept)
+        known[device][index].store(uint64_t(out->clusters4) << 32 | uint64_t(out->clusters8) << 16 | uint64_t(out->sms),
+                                   std::memory_order_release);
+    return cudaSuccess;
 }
 
-// Pairs that share a tile: as many as keep every tile's pairs on the GPU at once, with four steps or
-// more for each.  What counts is known here from above only: a tile for each expert, or row if those
+// Pairs that share a tile: as many as let every tile have a cluster on the GPU at once, with four steps
+// or more for each pair.  What counts is known here from above only: a tile for each expert, or row if those
 // are fewer, and one for every kMaxN rows; for the weight gradients, whose steps are an expert's
 // rows, their mean.
-template <Product P> int split_of(const ugdr_x_experts &m, int pairs) {
+template <Product P> int split_of(const ugdr_x_experts &m, const Residency &on) {
     const auto tiles_of = [](int64_t n, int64_t size) { return (n + size - 1) / size; };
     const int64_t features = P == kUp || P == kBack || P == kGradIn ? m.inner : m.hidden;
     int64_t tiles = tiles_of(features, kTileFeatures<P>), depth = 0;
@@ -1077,9 +1097,8 @@ template <Product P> int split_of(const ugdr_x_experts &m, int pairs) {
         tiles *= (m.rows < uint64_t(m.nexp) ? int64_t(m.rows) : m.nexp) + int64_t(m.rows / kMaxN);
         depth = P == kDown ? m.inner : P == kInput ? 2 * int64_t(m.inner) : m.hidden;
     }
-    for (int split = kMaxSplit; split > 1; split /= 2)
-        if (tiles * split <= pairs && depth >= 4 * split * kDepth) return split;
-    return 1;
+    if (tiles <= on.clusters8 && depth >= 16 * kDepth) return 4;
+    return tiles <= on.clusters4 && depth >= 8 * kDepth ? 2 : 1;
 }
 
 // One product.  `a` and `b` are its operands: the weights and the rows, or the two row tensors of a
@@ -1121,28 +1140,31 @@ cudaError_t launch(const ugdr_x_experts &m, const void *a, const void *b, void *
     }
     const Shape shape{m.counts, m.status, int(m.rows), m.nexp, m.hidden, m.inner, m.act, stages, stage_bytes};
 
-    int device = 0, sms = 0;
+    int device = 0;
     if (cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return e;
-    auto *kernel = expert_kernel<T, P>;
     constexpr int kIndex = int(P) * 2 + std::is_same_v<T, __half>;
-    if (cudaError_t e = prepare(reinterpret_cast<const void *>(kernel), device, kIndex, &sms); e != cudaSuccess) return e;
+    auto *kernel = expert_kernel<T, P>, *split_kernel = expert_split_kernel<T, P>;
+    Residency plain, clusters;
+    if (cudaError_t e = residency(reinterpret_cast<const void *>(kernel), false, device, kIndex, &plain); e != cudaSuccess)
+        return e;
+    if (cudaError_t e = residency(reinterpret_cast<const void *>(split_kernel), true, device, 12 + kIndex, &clusters);
+        e != cudaSuccess)
+        return e;
     cudaLaunchAttribute attributes[2] = {};
     attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attributes[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(unsigned(sms / 2 * 2));
+    config.gridDim = dim3(unsigned(plain.sms / 2 * 2));
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = shared_bytes(m.nexp);
     config.stream = s;
     config.attrs = attributes;
     config.numAttrs = 1;
-    if (const int split = split_of<P>(m, sms / 2); split > 1) {
-        kernel = expert_split_kernel<T, P>;
-        if (cudaError_t e = prepare(reinterpret_cast<const void *>(kernel), device, 12 + kIndex, &sms); e != cudaSuccess)
-            return e;
+    if (const int split = split_of<P>(m, clusters); split > 1) {
+        kernel = split_kernel;
         attributes[1].id = cudaLaunchAttributeClusterDimension;
         attributes[1].val.clusterDim = {unsigned(2 * split), 1, 1};
-        config.gridDim = dim3(unsigned(sms / (2 * split) * (2 * split)));
+        config.gridDim = dim3(unsigned(split == 4 ? 8 * clusters.clusters8 : 4 * clusters.clusters4));
         config.numAttrs = 2;
     }
     return cudaLaunchKernelEx(&config, kernel, maps, shape, static_cast<T *>(out), gu);
