@@ -926,10 +926,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     Loader<P> loader = loader_of<P>(maps, m, k);
     Issuer<T, P> issuer = issuer_of<T, P>(m, k);
     TailClearer clearer{m, sh, k};
-    float *sums = reinterpret_cast<float *>(k.ring);  // [part][column][feature], once the ring is idle
     uint32_t phase = 0;
 
-    while (tiles.next(t)) {
+    for (bool begun = false; tiles.next(t); begun = true) {
         const int steps = steps_of<P>(m, t.rows), k0 = steps * part / split, k1 = steps * (part + 1) / split;
         const int n = kWeightGrad<P> ? kMaxN : ceil_div(t.rows, kStepN) * kStepN, columns = n / split;  // each pair's
         const int feature = t.feature + int(k.rank) * (kTileFeatures<P> / 2);
@@ -945,7 +944,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         phase ^= uint32_t(k1 > k0);
         __syncthreads();
         const bool fine = !sh.aborted;
-        cluster_sync();  // every pair's products are over, and no load is under way
+        // The sums, [part][column][feature], go where the epilogue's staging is, or, if that is too
+        // small, into the ring, once every pair's products are over and no load is under way.
+        const bool apart = n * kStagingRow * 4 <= int(2 * kStagingBytes);
+        float *sums = apart ? k.staging : reinterpret_cast<float *>(k.ring);
+        if (begun || !apart) cluster_sync();
         fence_after();
         if (fine && warp >= 4 && k1 > k0) {
             const int quarter = warp % 4, group = warp / 4 - 1;
@@ -1082,10 +1085,10 @@ cudaError_t residency(const void *kernel, bool split, int device, int index, Res
     return cudaSuccess;
 }
 
-// Pairs that share a tile: as many as let every tile have a cluster on the GPU at once, with four steps
-// or more for each pair.  What counts is known here from above only: a tile for each expert, or row if those
-// are fewer, and one for every kMaxN rows; for the weight gradients, whose steps are an expert's
-// rows, their mean.
+// Pairs that share a tile: as many as let every tile have a cluster on the GPU at once, where the steps
+// are enough to gain by it.  What counts is known here from above only: a tile for each expert, or row
+// if those are fewer, and one for every kMaxN rows; for the weight gradients, whose steps are an
+// expert's rows, their mean.
 template <Product P> int split_of(const ugdr_x_experts &m, const Residency &on) {
     const auto tiles_of = [](int64_t n, int64_t size) { return (n + size - 1) / size; };
     const int64_t features = P == kUp || P == kBack || P == kGradIn ? m.inner : m.hidden;
@@ -1097,8 +1100,9 @@ template <Product P> int split_of(const ugdr_x_experts &m, const Residency &on) 
         tiles *= (m.rows < uint64_t(m.nexp) ? int64_t(m.rows) : m.nexp) + int64_t(m.rows / kMaxN);
         depth = P == kDown ? m.inner : P == kInput ? 2 * int64_t(m.inner) : m.hidden;
     }
-    if (tiles <= on.clusters8 && depth >= 16 * kDepth) return 4;
-    return tiles <= on.clusters4 && depth >= 8 * kDepth ? 2 : 1;
+    // Adding the parts up takes 2 to 3 us, a step 0.2 us.
+    if (tiles <= on.clusters8 && depth >= 20 * kDepth) return 4;
+    return tiles <= on.clusters4 && depth >= 28 * kDepth ? 2 : 1;
 }
 
 // One product.  `a` and `b` are its operands: the weights and the rows, or the two row tensors of a

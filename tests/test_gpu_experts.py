@@ -124,7 +124,7 @@ CASES = [
     ([15, 16, 17, 31, 32, 33], 136, 200), ([63, 64, 65, 127, 128, 129], 256, 128),
     ([255, 256, 257], 128, 264), ([511, 1, 513], 520, 136), ([700], 1000, 712),
     # few tiles and long sums, which pairs of CTAs share
-    ([2500], 144, 264), ([1100, 0, 31], 200, 72), ([33], 1160, 136), ([2], 72, 2056), ([700, 900], 72, 136),
+    ([2500], 144, 264), ([5, 40, 0, 300], 1800, 520), ([1900], 1032, 1032), ([1100, 0, 31], 200, 72), ([33], 1160, 136), ([2], 72, 2056), ([700, 900], 72, 136),
     ([1] * 40, 72, 520), ([2, 0, 300, 7, 0, 0, 90], 1032, 1416), ([130], 2048, 24), ([40, 9], 24, 2056),
 ]
 
