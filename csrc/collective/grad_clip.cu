@@ -22,7 +22,8 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kGroup = 8;    // elements a thread takes at once: 16 or 32 bytes
-constexpr int kInFlight = 16;  // 16 / element size groups in flight per thread: 128 bytes
+constexpr int kInFlight = 8;  // 8 / element size groups in flight per thread: 64 bytes
+constexpr int kBlocks = 4;    // per SM: some find their next tensor while the others read
 static_assert(kThreads * kGroup == kGradChunk, "one group per thread and chunk");
 
 template <int TYPE> struct Element;
@@ -202,7 +203,7 @@ __device__ __forceinline__ uint32_t share(uint32_t chunks, uint32_t block) {
     return uint32_t(uint64_t(chunks) * block / gridDim.x);
 }
 
-__global__ void __launch_bounds__(kThreads, 2) grad_norm_kernel(Plan p, uint32_t chunks, double *partials) {
+__global__ void __launch_bounds__(kThreads, kBlocks) grad_norm_kernel(Plan p, uint32_t chunks, double *partials) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t c1 = share(chunks, blockIdx.x + 1);
     uint32_t c = share(chunks, blockIdx.x);
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(kThreads) grad_sum_kernel(const double *partia
 template <int IN, int OUT> __device__ void span_scale(const ugdr_x_grad &t, uint32_t c0, uint32_t c1, float coef) {
     using T = typename Element<IN>::type;
     using O = typename Element<OUT>::type;
-    constexpr int kUnroll = 4;
+    constexpr int kUnroll = 2;
     const T *g = static_cast<const T *>(t.grad);
     O *out = static_cast<O *>(t.out);
     const uint32_t lead = lead_of(g);
@@ -279,7 +280,7 @@ template <int IN, int OUT> __device__ void span_scale(const ugdr_x_grad &t, uint
 
 // Every block sums the partial sums itself, in one order, so no block waits for another; then it
 // scales its run of chunks backwards: what the norm pass read last is what the L2 still holds.
-__global__ void __launch_bounds__(kThreads, 2) grad_scale_kernel(Plan p, uint32_t chunks, const double *partials,
+__global__ void __launch_bounds__(kThreads, kBlocks) grad_scale_kernel(Plan p, uint32_t chunks, const double *partials,
                                                                  int npartials, float max_norm, float *norm_out) {
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the norm kernel's sums are there
     const double norm = sqrt(partial_sum(partials, npartials));
@@ -317,12 +318,12 @@ Plan as_plan(const void *plan, int n) {
     return {grads, reinterpret_cast<const uint32_t *>(grads + n), n};
 }
 
-// Two blocks per SM, fewer when there are fewer chunks; at least one, which writes the sum or norm.
+// kBlocks blocks per SM, fewer when there are fewer chunks; at least one, which writes the sum or norm.
 int blocks_for(uint64_t chunks) {
     int device = 0, sms = 148;
     cudaGetDevice(&device);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    const uint64_t most = uint64_t(sms) * 2 < UGDR_X_GRAD_PARTIALS ? uint64_t(sms) * 2 : UGDR_X_GRAD_PARTIALS;
+    const uint64_t most = uint64_t(sms) * kBlocks < UGDR_X_GRAD_PARTIALS ? uint64_t(sms) * kBlocks : UGDR_X_GRAD_PARTIALS;
     return int(chunks < 1 ? 1 : chunks < most ? chunks : most);
 }
 
