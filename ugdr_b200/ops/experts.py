@@ -22,9 +22,8 @@ them, as it does when a bounded wait inside a kernel ran out.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
-from typing import NamedTuple
+from typing import Iterable, NamedTuple
 
 import torch
 
@@ -52,43 +51,37 @@ class ExpertFFNSaved(NamedTuple):
 _status: dict[int, torch.Tensor] = {}
 
 
+_bound: C.CDLL | None = None
+
+
 def _lib() -> C.CDLL:
-    L = N.lib()
-    if not getattr(L, "_expert_sigs", False):
-        vp = C.c_void_p
+    global _bound
+    if _bound is None:
+        L, vp = N.lib(), C.c_void_p
         L.ugdr_x_expert_ffn.restype = C.c_int
         L.ugdr_x_expert_ffn.argtypes = [C.POINTER(_Experts)] + [vp] * 5
         L.ugdr_x_expert_ffn_backward.restype = C.c_int
         L.ugdr_x_expert_ffn_backward.argtypes = [C.POINTER(_Experts)] + [vp] * 9
-        L._expert_sigs = True
-    return L
+        _bound = L
+    return _bound
 
 
-class _On:
-    """The tensors' device current, and `stream` the one that outputs and scratch are allocated for;
-    as a context, the raw stream.  A class, and the raw stream without a Stream object: the calls
-    around it take a few microseconds."""
-
-    __slots__ = ("device", "stream", "guards")
-
-    def __init__(self, device: torch.device, stream: torch.cuda.Stream | None):
-        if stream is not None and stream.device != device:
-            raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
-        self.device, self.stream, self.guards = device, stream, None
-
-    def __enter__(self) -> int:
-        if self.stream is None and torch.cuda.current_device() == self.device.index:
-            return torch._C._cuda_getCurrentRawStream(self.device.index)
-        self.guards = contextlib.ExitStack()
-        self.guards.enter_context(torch.cuda.device(self.device))
-        if self.stream is None:
-            return torch._C._cuda_getCurrentRawStream(self.device.index)
-        self.guards.enter_context(torch.cuda.stream(self.stream))
-        return self.stream.cuda_stream
-
-    def __exit__(self, *exc) -> None:
-        if self.guards is not None:
-            self.guards.close()
+def _enqueue(device: torch.device, stream: torch.cuda.Stream | None, tensors: Iterable[torch.Tensor], call):
+    """call(raw stream) with the tensors' device current and `stream` (default: the device's current
+    one) the stream that outputs and scratch are allocated for.  On a stream of the caller's choice the
+    tensors' memory is kept from reuse until the stream is through with it."""
+    if stream is None:
+        if torch.cuda.current_device() == device.index:  # the short way
+            return call(torch._C._cuda_getCurrentRawStream(device.index))
+        with torch.cuda.device(device):
+            return call(torch._C._cuda_getCurrentRawStream(device.index))
+    if stream.device != device:
+        raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+    with torch.cuda.device(device), torch.cuda.stream(stream):
+        result = call(stream.cuda_stream)
+    for t in tensors:
+        t.record_stream(stream)
+    return result
 
 
 def _status_word(device: torch.device) -> torch.Tensor:
@@ -116,12 +109,10 @@ def check_status(device: torch.device | int | None = None) -> None:
                             2: "expert counts are negative or exceed the rows"}.get(st, f"status {st}"))
 
 
-def _rows(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor, dtype: torch.dtype | None = None
-          ) -> tuple[int, int]:
-    """The addresses that t begins and ends at, checked to be a dense tensor of that shape beside `like`."""
-    dtype = dtype or like.dtype
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != like.device:
-        raise ValueError(f"{name} must be a {dtype} tensor on {like.device}")
+def _span(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype, device: torch.device) -> tuple[int, int]:
+    """The addresses that t begins and ends at, checked to be a dense tensor as described."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be a {dtype} tensor on {device}")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     at = t.data_ptr()
@@ -137,9 +128,10 @@ def _checked(x, counts, w_in, w_out, act: str) -> tuple[_Experts, dict[str, tupl
     if act not in _ACTS:
         raise ValueError(f"act must be one of {sorted(_ACTS)}, got {act!r}")
     rows, hidden = x.shape
+    dtype, device = x.dtype, x.device
     if not isinstance(counts, torch.Tensor) or counts.dtype != torch.int32 or counts.dim() != 1 \
-            or counts.device != x.device or not counts.is_contiguous():
-        raise ValueError(f"counts must be a contiguous int32 tensor [experts] on {x.device}")
+            or counts.device != device or not counts.is_contiguous():
+        raise ValueError(f"counts must be a contiguous int32 tensor [experts] on {device}")
     nexp = counts.shape[0]
     if not 1 <= nexp <= MAX_EXPERTS:
         raise ValueError(f"1..{MAX_EXPERTS} experts supported, got {nexp}")
@@ -151,10 +143,10 @@ def _checked(x, counts, w_in, w_out, act: str) -> tuple[_Experts, dict[str, tupl
     if rows >= 1 << 31:
         raise ValueError(f"at most 2**31 - 1 rows, got {rows}")
     at = counts.data_ptr()
-    spans = {"x": _rows(x, "x", (rows, hidden), x), "counts": (at, at + 4 * nexp),
-             "w_in": _rows(w_in, "w_in", (nexp, 2, inner, hidden), x),
-             "w_out": _rows(w_out, "w_out", (nexp, hidden, inner), x)}
-    return _Experts(at, spans["w_in"][0], spans["w_out"][0], None, rows, nexp, hidden, inner, _TYPES[x.dtype],
+    spans = {"x": _span(x, "x", x.shape, dtype, device), "counts": (at, at + 4 * nexp),
+             "w_in": _span(w_in, "w_in", (nexp, 2, inner, hidden), dtype, device),
+             "w_out": _span(w_out, "w_out", (nexp, hidden, inner), dtype, device)}
+    return _Experts(at, spans["w_in"][0], spans["w_out"][0], None, rows, nexp, hidden, inner, _TYPES[dtype],
                     _ACTS[act]), spans
 
 
@@ -170,15 +162,19 @@ def _apart(name: str, span: tuple[int, int], others: dict[str, tuple[int, int]],
 def _forward(x, counts, w_in, w_out, act, out, stream, train):
     m, spans = _checked(x, counts, w_in, w_out, act)
     if out is not None:
-        _apart("out", _rows(out, "out", x.shape, x), spans, () if train else ("x",))
-    with _On(x.device, stream) as s:
+        spans_out = _span(out, "out", x.shape, x.dtype, x.device)
+        _apart("out", spans_out, spans, () if train else ("x",))
+
+    def call(s):
         m.status = _status_word(x.device).data_ptr()
         y = x.new_empty(x.shape) if out is None else out
         h = x.new_empty((m.rows, m.inner))
         gu = x.new_empty((m.rows, 2, m.inner), dtype=torch.float32) if train else None
-        check(_lib().ugdr_x_expert_ffn(C.byref(m), x.data_ptr(), y.data_ptr(), h.data_ptr(),
-                                       gu.data_ptr() if train else None, s), "ugdr_x_expert_ffn")
-    return y, ExpertFFNSaved(h, gu) if train else None
+        check(_lib().ugdr_x_expert_ffn(m, spans["x"][0], y.data_ptr(), h.data_ptr(), gu.data_ptr() if train else None,
+                                       s), "ugdr_x_expert_ffn")
+        return y, ExpertFFNSaved(h, gu) if train else None
+
+    return _enqueue(x.device, stream, (x, counts, w_in, w_out) if out is None else (x, counts, w_in, w_out, out), call)
 
 
 def expert_ffn(x: torch.Tensor, counts: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, act: str = "silu",
@@ -205,23 +201,29 @@ def expert_ffn_backward(dy: torch.Tensor, x: torch.Tensor, counts: torch.Tensor,
     given for them.  dx may be dy or x itself.  Weight gradients of experts without rows are
     zeros."""
     m, spans = _checked(x, counts, w_in, w_out, act)
-    spans["dy"] = _rows(dy, "dy", x.shape, x)
-    spans["saved.h"] = _rows(saved.h, "saved.h", (m.rows, m.inner), x)
-    spans["saved.gu"] = _rows(saved.gu, "saved.gu", (m.rows, 2, m.inner), x, torch.float32)
+    dtype, device = x.dtype, x.device
+    spans["dy"] = _span(dy, "dy", x.shape, dtype, device)
+    spans["saved.h"] = _span(saved.h, "saved.h", (m.rows, m.inner), dtype, device)
+    spans["saved.gu"] = _span(saved.gu, "saved.gu", (m.rows, 2, m.inner), torch.float32, device)
     if spans["saved.gu"][0] % 32:
         raise ValueError("saved.gu must be 32-byte aligned")
-    for name, t, like in (("dx", dx, x), ("dw_in", dw_in, w_in), ("dw_out", dw_out, w_out)):
+    tensors = [x, counts, w_in, w_out, dy, saved.h, saved.gu]
+    for name, t, shape in (("dx", dx, x.shape), ("dw_in", dw_in, w_in.shape), ("dw_out", dw_out, w_out.shape)):
         if t is not None:
-            span = _rows(t, name, like.shape, x)
+            span = _span(t, name, shape, dtype, device)
             _apart(name, span, spans, ("dy", "x") if name == "dx" else ())
             spans[name] = span
-    with _On(x.device, stream) as s:
-        m.status = _status_word(x.device).data_ptr()
-        dx = x.new_empty(x.shape) if dx is None else dx
-        dw_in = x.new_empty(w_in.shape) if dw_in is None else dw_in
-        dw_out = x.new_empty(w_out.shape) if dw_out is None else dw_out
+            tensors.append(t)
+
+    def call(s):
+        m.status = _status_word(device).data_ptr()
+        gx = x.new_empty(x.shape) if dx is None else dx
+        gin = x.new_empty(w_in.shape) if dw_in is None else dw_in
+        gout = x.new_empty(w_out.shape) if dw_out is None else dw_out
         dgu = x.new_empty((m.rows, 2, m.inner))
-        check(_lib().ugdr_x_expert_ffn_backward(C.byref(m), spans["dy"][0], spans["x"][0], spans["saved.h"][0],
-                                                spans["saved.gu"][0], dgu.data_ptr(), dx.data_ptr(),
-                                                dw_in.data_ptr(), dw_out.data_ptr(), s), "ugdr_x_expert_ffn_backward")
-    return dx, dw_in, dw_out
+        check(_lib().ugdr_x_expert_ffn_backward(m, spans["dy"][0], spans["x"][0], spans["saved.h"][0],
+                                                spans["saved.gu"][0], dgu.data_ptr(), gx.data_ptr(), gin.data_ptr(),
+                                                gout.data_ptr(), s), "ugdr_x_expert_ffn_backward")
+        return gx, gin, gout
+
+    return _enqueue(device, stream, tensors, call)

@@ -15,7 +15,7 @@ import torch
 
 from .. import _native as N
 from ..parallel.peers import check
-from .experts import _On
+from .experts import _enqueue
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 PARTIALS = 2048
@@ -26,10 +26,13 @@ class _Grad(C.Structure):
                 ("out_type", C.c_int32)]
 
 
+_bound: C.CDLL | None = None
+
+
 def _lib() -> C.CDLL:
-    L = N.lib()
-    if not getattr(L, "_grad_sigs", False):
-        vp, i, u64 = C.c_void_p, C.c_int, C.c_uint64
+    global _bound
+    if _bound is None:
+        L, vp, i, u64 = N.lib(), C.c_void_p, C.c_int, C.c_uint64
         L.ugdr_x_grad_plan_bytes.restype = C.c_size_t
         L.ugdr_x_grad_plan_bytes.argtypes = [i]
         L.ugdr_x_grad_plan.restype = i
@@ -38,8 +41,8 @@ def _lib() -> C.CDLL:
         L.ugdr_x_grad_sum_squares.argtypes = [vp, i, u64, vp, vp, vp]
         L.ugdr_x_grad_clip.restype = i
         L.ugdr_x_grad_clip.argtypes = [vp, i, u64, vp, vp, C.c_float, vp, vp]
-        L._grad_sigs = True
-    return L
+        _bound = L
+    return _bound
 
 
 class GradClip:
@@ -108,12 +111,14 @@ class GradClip:
 
     def sum_squares(self, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
         """The sum of the squares of all elements, a float64 tensor on the device."""
-        with _On(self.device, stream) as s:
+        def call(s):
             partials = self._plan.new_empty(PARTIALS, dtype=torch.float64)
             total = self._plan.new_empty((), dtype=torch.float64)
             check(_lib().ugdr_x_grad_sum_squares(self._plan.data_ptr(), self._n, self._chunks, partials.data_ptr(),
                                                  total.data_ptr(), s), "ugdr_x_grad_sum_squares")
-        return total
+            return total
+
+        return _enqueue(self.device, stream, (self._plan, *self.grads), call)
 
     def clip(self, max_norm: float, sum_squares: torch.Tensor | None = None,
              stream: torch.cuda.Stream | None = None) -> torch.Tensor:
@@ -127,10 +132,13 @@ class GradClip:
         if sum_squares is not None and (not isinstance(sum_squares, torch.Tensor) or sum_squares.numel() != 1
                                         or sum_squares.dtype != torch.float64 or sum_squares.device != self.device):
             raise ValueError(f"sum_squares must be one float64 on {self.device}")
-        with _On(self.device, stream) as s:
+        def call(s):
             partials = self._plan.new_empty(PARTIALS, dtype=torch.float64)
             norm = self._plan.new_empty((), dtype=torch.float32)
             check(_lib().ugdr_x_grad_clip(self._plan.data_ptr(), self._n, self._chunks, partials.data_ptr(),
                                           None if sum_squares is None else sum_squares.data_ptr(), max_norm,
                                           norm.data_ptr(), s), "ugdr_x_grad_clip")
-        return norm
+            return norm
+
+        return _enqueue(self.device, stream, (self._plan, *self.grads, *self.out,
+                                              *(() if sum_squares is None else (sum_squares,))), call)
