@@ -10,8 +10,9 @@ bool aligned32(const void *p) { return p != nullptr && reinterpret_cast<uintptr_
 
 bool valid(const ugdr_x_experts *m) {
     return m != nullptr && m->counts != nullptr && m->status != nullptr && aligned16(m->w_in) && aligned16(m->w_out) &&
-           m->rows <= INT32_MAX && m->nexp >= 1 && m->nexp <= UGDR_X_EXPERTS_MAX && m->hidden >= 8 &&
-           m->hidden % 8 == 0 && m->inner >= 8 && m->inner % 8 == 0 &&
+           m->rows <= UGDR_X_EXPERTS_MAX_ROWS && m->nexp >= 1 && m->nexp <= UGDR_X_EXPERTS_MAX && m->hidden >= 8 &&
+           m->hidden <= UGDR_X_EXPERTS_MAX_SIZE && m->hidden % 8 == 0 && m->inner >= 8 &&
+           m->inner <= UGDR_X_EXPERTS_MAX_SIZE && m->inner % 8 == 0 &&
            (m->type == UGDR_X_TYPE_BF16 || m->type == UGDR_X_TYPE_FP16) &&
            (m->act == UGDR_X_ACT_SILU || m->act == UGDR_X_ACT_GELU);
 }

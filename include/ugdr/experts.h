@@ -22,12 +22,16 @@ extern "C" {
 #define UGDR_X_ACT_SILU 0 /* a(g) = g / (1 + exp(-g)) */
 #define UGDR_X_ACT_GELU 1 /* a(g) = g (1 + erf(g / sqrt 2)) / 2 */
 
-#define UGDR_X_EXPERTS_MAX 4096
+#define UGDR_X_EXPERTS_MAX 4096             /* experts */
+#define UGDR_X_EXPERTS_MAX_ROWS (1u << 28)   /* rows of a call */
+#define UGDR_X_EXPERTS_MAX_SIZE (1 << 20)    /* hidden and inner */
 
 /* A rank's experts and the grouping of the rows: expert e's rows are the counts[e] rows after those
  * of experts 0 .. e - 1.  The counts are read on the device, so no call waits for the host; rows
  * behind the last group are neither read for a result nor written.  Tensors are contiguous and
- * 16-byte aligned, hidden and inner multiples of 8, type BF16 or FP16 (accumulation is fp32).
+ * 16-byte aligned, hidden and inner multiples of 8, type BF16 or FP16.  Sums are fp32; h, dg and du
+ * are rounded to the type once, as operands of the next product (so with FP16 they must stay within
+ * its range, as x and y must).
  * *status (a device word, not cleared by the calls) becomes 1 when a bounded wait inside a kernel
  * ran out and 2 when a count is negative or the counts add up to more than `rows`; negative counts
  * then count as 0 and rows past `rows` are dropped. */

@@ -226,6 +226,56 @@ def test_two_streams_at_once():
             assert all(torch.equal(w[k], g[k]) for k in w)
 
 
+def test_inputs_on_a_chosen_stream_are_kept_until_it_is_through():
+    """Inputs dropped right after the call: their memory is not given out while a busy stream has
+    yet to read them."""
+    from ugdr_b200 import ops
+
+    x, c, w_in, w_out, _ = inputs([64, 64], 256, 256, torch.bfloat16)
+    want = ops.expert_ffn(x, c, w_in, w_out)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        again = x.clone()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)  # some 10 ms
+        got = ops.expert_ffn(again, c, w_in, w_out, stream=side)
+        del again
+        others = [torch.full_like(x, float("nan")) for _ in range(4)]
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        del others
+
+
+def test_another_device_than_the_current_one():
+    if gpu_count() < 2:
+        pytest.skip("needs 2 GPUs")
+    x, c, w_in, w_out, dy = (t.to("cuda:1") for t in inputs([20, 45], 72, 136, torch.bfloat16))
+    got = step(x, c, w_in, w_out, "silu", dy)
+    assert torch.cuda.current_device() == 0 and all(t.device.index == 1 for t in got.values())
+    compare(x, c, w_in, w_out, "silu", dy, got)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^32 elements kept for the backward pass: the first and the last rows are right, and
+    the weights' gradients when only the last rows have one."""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of free GPU memory")
+    rows, hidden, inner = 70_001, 64, 32_768
+    x, c, w_in, w_out, dy = inputs([rows - 3, 3], hidden, inner, torch.bfloat16)
+    dy[:rows - 7] = 0
+    got = step(x, c, w_in, w_out, "silu", dy)
+    assert 2 * rows * inner > 1 << 32
+    for e, r in ((0, slice(0, 5)), (0, slice(rows - 7, rows - 3)), (1, slice(rows - 3, rows))):
+        o = oracle(x[r], w_in[e], w_out[e], "silu", dy[r])
+        near(got["y"][r], *o["y"], "y")
+        near(got["dx"][r], *o["dx"], "dx")
+        if r.start > 5:
+            near(got["dw_in"][e], *o["dw_in"], "dw_in")
+            near(got["dw_out"][e], *o["dw_out"], "dw_out")
+
+
 def test_captured_steps_follow_their_inputs():
     """Two graphs of a training step, replayed in turn with new rows and new counts."""
     sets = [inputs([20, 100], 136, 136, torch.bfloat16, seed=k) for k in (1, 2)]

@@ -194,6 +194,19 @@ def test_after_an_allreduce_in_the_symmetric_buffer():
     check_scaled([flat], [before], 2.0 / (want + 1e-6))
 
 
+def test_more_than_2_to_the_32_elements():
+    from ugdr_b200.ops import GradClip
+
+    n = (1 << 32) + 4101
+    if torch.cuda.mem_get_info()[0] < 3 * n:
+        pytest.skip("needs 13 GB of free GPU memory")
+    g = torch.full((n,), 2.0 ** -8, dtype=torch.bfloat16, device="cuda")
+    want = math.sqrt(n) * 2.0 ** -8
+    assert abs(float(GradClip([g]).clip(want / 4)) - want) <= NORM_REL * want
+    for part in (g[:5000], g[1 << 31:(1 << 31) + 5000], g[-5000:]):
+        assert bool((part == 2.0 ** -10).all())
+
+
 def test_refusals():
     from ugdr_b200.ops import GradClip
 

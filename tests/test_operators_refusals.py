@@ -20,7 +20,7 @@ def _experts(**change):
 
 @pytest.mark.parametrize("change", [
     dict(counts=None), dict(w_in=None), dict(w_out=None), dict(status=None), dict(w_in=0x2008), dict(w_out=0x3004),
-    dict(rows=1 << 31), dict(nexp=0), dict(nexp=4097), dict(hidden=0), dict(hidden=12), dict(hidden=-8),
+    dict(rows=(1 << 28) + 1), dict(rows=1 << 40), dict(hidden=(1 << 20) + 8), dict(inner=1 << 21), dict(nexp=0), dict(nexp=4097), dict(hidden=0), dict(hidden=12), dict(hidden=-8),
     dict(inner=0), dict(inner=20), dict(type=2), dict(type=-1), dict(act=2), dict(act=-1)])
 def test_the_block_refuses_what_it_cannot_do(change):
     from ugdr_b200.ops.experts import _lib

@@ -6,8 +6,9 @@ in the receive area (`MoEAllToAll.recv_view()` with `MoEAllToAll.expert_rows()`)
 with every row's own expert's weights.  Serving calls `expert_ffn`; a training step calls
 `expert_ffn_train`, which keeps what the backward pass needs, and `expert_ffn_backward`.
 
-Tensors are contiguous CUDA tensors on one device, bfloat16 or float16 throughout (products and
-sums in fp32):
+Tensors are contiguous CUDA tensors on one device, bfloat16 or float16 throughout; sums are fp32, and
+h, dg and du are rounded to the type once, as operands of the next product (so with float16 they
+must stay within its range, as x and y must):
 
     x, y, dy, dx   [rows, hidden]             hidden and inner multiples of 8
     counts         [experts] int32            rows of each expert, in order; read on the device
@@ -33,6 +34,8 @@ from ..parallel.peers import check
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
 _ACTS = {"silu": 0, "gelu": 1}
 MAX_EXPERTS = 4096
+MAX_ROWS = 1 << 28
+MAX_SIZE = 1 << 20  # of hidden and inner
 
 
 class _Experts(C.Structure):
@@ -89,8 +92,9 @@ def _status_word(device: torch.device) -> torch.Tensor:
     if word is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("call an expert operator once on this device before capturing it into a graph")
-        word = _status[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+        word = torch.zeros(1, dtype=torch.int32, device=device)
         torch.cuda.current_stream(device).synchronize()  # zero before any stream may write it
+        word = _status.setdefault(device.index, word)
     return word
 
 
@@ -138,10 +142,10 @@ def _checked(x, counts, w_in, w_out, act: str) -> tuple[_Experts, dict[str, tupl
     if not isinstance(w_out, torch.Tensor) or w_out.dim() != 3:
         raise ValueError("w_out must be a tensor [experts, hidden, inner]")
     inner = w_out.shape[2]
-    if hidden < 8 or hidden % 8 or inner < 8 or inner % 8:
-        raise ValueError(f"hidden and inner must be multiples of 8, got {hidden} and {inner}")
-    if rows >= 1 << 31:
-        raise ValueError(f"at most 2**31 - 1 rows, got {rows}")
+    if not 8 <= hidden <= MAX_SIZE or hidden % 8 or not 8 <= inner <= MAX_SIZE or inner % 8:
+        raise ValueError(f"hidden and inner must be multiples of 8 up to {MAX_SIZE}, got {hidden} and {inner}")
+    if rows > MAX_ROWS:
+        raise ValueError(f"at most {MAX_ROWS} rows, got {rows}")
     at = counts.data_ptr()
     spans = {"x": _span(x, "x", x.shape, dtype, device), "counts": (at, at + 4 * nexp),
              "w_in": _span(w_in, "w_in", (nexp, 2, inner, hidden), dtype, device),
