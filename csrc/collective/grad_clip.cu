@@ -27,7 +27,7 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kGroup = 8;    // elements a thread takes at once: 16 or 32 bytes
 constexpr int kInFlight = 8;  // 8 / element size groups in flight per thread: 64 bytes
-constexpr int kBlocks = 4;    // per SM: some find their next tensor while the others read
+constexpr int kNormBlocks = 3, kScaleBlocks = 2;  // per SM: some find their next tensor while the others read
 static_assert(kThreads * kGroup == kGradChunk, "one group per thread and chunk");
 
 template <int TYPE> struct Element;
@@ -149,15 +149,25 @@ template <typename T> __device__ __forceinline__ uint32_t lead_of(const T *p) {
     return uint32_t(reinterpret_cast<uintptr_t>(p) % (sizeof(T) * kGroup) / sizeof(T));
 }
 
-// The chunks of [c0, c1) that lie in the tensor as a whole: [whole.a, whole.b).  At most the first
-// and the last do not.
-struct Whole {
+// The chunks of [c0, c1) in which this thread's group lies in the tensor as a whole: [a, b).
+struct Mine {
     uint32_t a, b;
 };
-__device__ __forceinline__ Whole whole_chunks(uint32_t c0, uint32_t c1, uint32_t lead, uint64_t n) {
-    const uint32_t a = c0 == 0 && lead != 0 ? 1 : c0;
-    const uint32_t b = uint32_t(min(uint64_t(c1), (n + lead) / kGradChunk));
-    return {min(a, c1), max(min(a, c1), b)};
+__device__ __forceinline__ Mine my_chunks(uint32_t c0, uint32_t c1, uint32_t lead, int64_t n) {
+    const uint32_t a = c0 + (c0 == 0 && lead != 0 && threadIdx.x == 0);
+    const int64_t last = n + lead - kGroup * int64_t(threadIdx.x + 1);  // begins no further than here
+    const uint32_t b = last < 0 ? a : uint32_t(min(int64_t(c1), last / kGradChunk + 1));
+    return {a, max(a, b)};
+}
+
+// The elements outside whole groups, before the first and behind the last: f(index), from the thread
+// and the chunk that they belong to.
+template <typename F> __device__ __forceinline__ void partial_groups(uint32_t c0, uint32_t c1, uint32_t lead, int64_t n, F f) {
+    if (c0 == 0 && lead != 0 && threadIdx.x == 0)
+        for (int64_t i = 0; i < min(int64_t(kGroup - lead), n); ++i) f(i);
+    const int64_t groups = (n + lead) / kGroup, chunk = groups / kThreads;
+    if (chunk >= c0 && chunk < c1 && threadIdx.x == uint32_t(groups % kThreads) && groups * kGroup >= lead)
+        for (int64_t i = groups * kGroup - lead; i < n; ++i) f(i);
 }
 
 // The squares of the chunks [c0, c1) of one tensor.
@@ -167,11 +177,11 @@ template <int TYPE> __device__ double span_squares(const ugdr_x_grad &t, uint32_
     const T *g = static_cast<const T *>(t.grad);
     const uint32_t lead = lead_of(g);
     const int64_t n = int64_t(t.count);
-    const Whole w = whole_chunks(c0, c1, lead, t.count);
+    const Mine w = my_chunks(c0, c1, lead, n);
     const T *p = g + (int64_t(w.a) * kGradChunk + threadIdx.x * kGroup - int64_t(lead));
     double acc = 0;
-    uint32_t c = w.a;
-    for (; c + kUnroll <= w.b; c += kUnroll, p += kUnroll * kGradChunk) {
+    int left = int(w.b - w.a);
+    for (; left >= kUnroll; left -= kUnroll, p += kUnroll * kGradChunk) {
         Group<T> v[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) v[u] = load_group(p + u * kGradChunk);
@@ -185,21 +195,21 @@ template <int TYPE> __device__ double span_squares(const ugdr_x_grad &t, uint32_
         }
         acc += wide ? squares_wide(p, kUnroll) : sum;
     }
-    for (; c < w.b; ++c, p += kGradChunk) {
-        const float q = squares(load_group(p));
-        acc += unsafe(q) ? squares_wide(p, 1) : double(q);
-    }
-    for (uint32_t edge = c0; edge < c1; ++edge) {
-        if (edge == w.a && w.a < w.b) edge = w.b;
-        if (edge == c1) break;
-        // Neighbours to neighbouring threads, and every square in fp64.
-        const int64_t at = int64_t(edge) * kGradChunk - int64_t(lead) + threadIdx.x;
+    if (left > 0) {  // at once too: the last of them stands in for those missing
+        Group<T> v[kUnroll];
 #pragma unroll
-        for (int j = 0; j < kGroup; ++j) {
-            const int64_t i = at + j * kThreads;
-            if (i >= 0 && i < n) acc = squares_wide(to_float(g[i]), acc);
+        for (int u = 0; u < kUnroll; ++u) v[u] = load_group(p + min(u, left - 1) * kGradChunk);
+        double sum = 0;
+        bool wide = false;
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const float q = squares(v[u]);
+            wide |= unsafe(q);
+            sum += u < left ? double(q) : 0.0;
         }
+        acc += wide ? squares_wide(p, left) : sum;
     }
+    partial_groups(c0, c1, lead, n, [&](int64_t i) { acc = squares_wide(to_float(g[i]), acc); });
     return acc;
 }
 
@@ -207,7 +217,7 @@ __device__ __forceinline__ uint32_t share(uint32_t chunks, uint32_t block) {
     return uint32_t(uint64_t(chunks) * block / gridDim.x);
 }
 
-__global__ void __launch_bounds__(kThreads, kBlocks) grad_norm_kernel(Plan p, uint32_t chunks, double *partials) {
+__global__ void __launch_bounds__(kThreads, kNormBlocks) grad_norm_kernel(Plan p, uint32_t chunks, double *partials) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t c1 = share(chunks, blockIdx.x + 1);
     uint32_t c = share(chunks, blockIdx.x);
@@ -245,27 +255,26 @@ __global__ void __launch_bounds__(kThreads) grad_sum_kernel(const double *partia
 template <int IN, int OUT> __device__ void span_scale(const ugdr_x_grad &t, uint32_t c0, uint32_t c1, float coef) {
     using T = typename Element<IN>::type;
     using O = typename Element<OUT>::type;
-    constexpr int kUnroll = 2;
+    constexpr int kUnroll = 4;
     const T *g = static_cast<const T *>(t.grad);
     O *out = static_cast<O *>(t.out);
     const uint32_t lead = lead_of(g);
-    const int64_t n = int64_t(t.count), mine = int64_t(threadIdx.x * kGroup) - int64_t(lead);
-    Whole w = whole_chunks(c0, c1, lead, t.count);
-    if (lead_of(out) != lead) w.b = w.a;  // whole groups of the output are not aligned
-    for (uint32_t edge = c0; edge < c1; ++edge) {
-        if (edge == w.a && w.a < w.b) edge = w.b;
-        if (edge == c1) break;
-        // Neighbours to neighbouring threads.
-        const int64_t at = int64_t(edge) * kGradChunk - int64_t(lead) + threadIdx.x;
+    const int64_t n = int64_t(t.count);
+    const auto one = [&](int64_t i) { from_float(out[i], to_float(g[i]) * coef); };
+    if (lead_of(out) != lead) {  // whole groups of the output are not aligned: neighbours to neighbouring threads
+        for (uint32_t c = c0; c < c1; ++c) {
+            const int64_t at = int64_t(c) * kGradChunk - int64_t(lead) + threadIdx.x;
 #pragma unroll
-        for (int j = 0; j < kGroup; ++j) {
-            const int64_t i = at + j * kThreads;
-            if (i >= 0 && i < n) from_float(out[i], to_float(g[i]) * coef);
+            for (int j = 0; j < kGroup; ++j)
+                if (at + j * kThreads >= 0 && at + j * kThreads < n) one(at + j * kThreads);
         }
+        return;
     }
-    const T *p = g + (int64_t(w.b) * kGradChunk + mine);
-    O *o = out + (int64_t(w.b) * kGradChunk + mine);
-    uint32_t left = w.b - w.a;
+    const Mine w = my_chunks(c0, c1, lead, n);
+    const int64_t begin = int64_t(w.b) * kGradChunk + threadIdx.x * kGroup - int64_t(lead);
+    const T *p = g + begin;
+    O *o = out + begin;
+    int left = int(w.b - w.a);
     for (; left >= kUnroll; left -= kUnroll) {
         Group<T> v[kUnroll];
         p -= kUnroll * kGradChunk;
@@ -275,16 +284,20 @@ template <int IN, int OUT> __device__ void span_scale(const ugdr_x_grad &t, uint
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) store_group(o + u * kGradChunk, scaled<O>(v[u], coef));
     }
-    for (; left > 0; --left) {
-        p -= kGradChunk;
-        o -= kGradChunk;
-        store_group(o, scaled<O>(load_group(p), coef));
+    if (left > 0) {
+        Group<T> v[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) v[u] = load_group(p - min(u + 1, left) * kGradChunk);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+            if (u < left) store_group(o - (u + 1) * kGradChunk, scaled<O>(v[u], coef));
     }
+    partial_groups(c0, c1, lead, n, one);
 }
 
 // Every block sums the partial sums itself, in one order, so no block waits for another; then it
 // scales its run of chunks backwards: what the norm pass read last is what the L2 still holds.
-__global__ void __launch_bounds__(kThreads, kBlocks) grad_scale_kernel(Plan p, uint32_t chunks, const double *partials,
+__global__ void __launch_bounds__(kThreads, kScaleBlocks) grad_scale_kernel(Plan p, uint32_t chunks, const double *partials,
                                                                  int npartials, float max_norm, float *norm_out) {
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the norm kernel's sums are there
     const double norm = sqrt(partial_sum(partials, npartials));
@@ -322,12 +335,13 @@ Plan as_plan(const void *plan, int n) {
     return {grads, reinterpret_cast<const uint32_t *>(grads + n), n};
 }
 
-// kBlocks blocks per SM, fewer when there are fewer chunks; at least one, which writes the sum or norm.
-int blocks_for(uint64_t chunks) {
+// As many blocks as the SMs hold, fewer when there are fewer chunks; at least one, which writes the sum
+// or the norm.
+int blocks_for(uint64_t chunks, int per_sm) {
     int device = 0, sms = 148;
     cudaGetDevice(&device);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    const uint64_t most = uint64_t(sms) * kBlocks < UGDR_X_GRAD_PARTIALS ? uint64_t(sms) * kBlocks : UGDR_X_GRAD_PARTIALS;
+    const uint64_t most = uint64_t(sms) * per_sm < UGDR_X_GRAD_PARTIALS ? uint64_t(sms) * per_sm : UGDR_X_GRAD_PARTIALS;
     return int(chunks < 1 ? 1 : chunks < most ? chunks : most);
 }
 
@@ -345,7 +359,7 @@ int grad_kernels(const KernelRef **out) {
 
 int launch_grad_sum_squares(const void *plan, int n, uint64_t chunks, double *partials, double *sum_squares,
                             cudaStream_t s) {
-    const int blocks = blocks_for(chunks);
+    const int blocks = blocks_for(chunks, kNormBlocks);
     grad_norm_kernel<<<blocks, kThreads, 0, s>>>(as_plan(plan, n), uint32_t(chunks), partials);
     grad_sum_kernel<<<1, kThreads, 0, s>>>(partials, blocks, sum_squares);
     return int(cudaGetLastError());
@@ -353,7 +367,7 @@ int launch_grad_sum_squares(const void *plan, int n, uint64_t chunks, double *pa
 
 int launch_grad_clip(const void *plan, int n, uint64_t chunks, double *partials, const double *sum_squares,
                      float max_norm, float *norm_out, cudaStream_t s) {
-    const int blocks = blocks_for(chunks);
+    const int blocks = blocks_for(chunks, kNormBlocks);
     if (sum_squares == nullptr)
         grad_norm_kernel<<<blocks, kThreads, 0, s>>>(as_plan(plan, n), uint32_t(chunks), partials);
     // Launched while the norm kernel runs: its blocks start as those of the norm kernel end.
@@ -361,7 +375,7 @@ int launch_grad_clip(const void *plan, int n, uint64_t chunks, double *partials,
     programmatic.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     programmatic.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(unsigned(blocks));
+    config.gridDim = dim3(unsigned(blocks_for(chunks, kScaleBlocks)));
     config.blockDim = dim3(kThreads);
     config.stream = s;
     config.attrs = &programmatic;
