@@ -171,7 +171,7 @@ def _forward(x, counts, w_in, w_out, act, out, stream, train):
 
     def call(s):
         m.status = _status_word(x.device).data_ptr()
-        y = x.new_empty(x.shape) if out is None else out
+        y = torch.empty_like(x) if out is None else out
         h = x.new_empty((m.rows, m.inner))
         gu = x.new_empty((m.rows, 2, m.inner), dtype=torch.float32) if train else None
         check(_lib().ugdr_x_expert_ffn(m, spans["x"][0], y.data_ptr(), h.data_ptr(), gu.data_ptr() if train else None,
@@ -221,9 +221,9 @@ def expert_ffn_backward(dy: torch.Tensor, x: torch.Tensor, counts: torch.Tensor,
 
     def call(s):
         m.status = _status_word(device).data_ptr()
-        gx = x.new_empty(x.shape) if dx is None else dx
-        gin = x.new_empty(w_in.shape) if dw_in is None else dw_in
-        gout = x.new_empty(w_out.shape) if dw_out is None else dw_out
+        gx = torch.empty_like(x) if dx is None else dx
+        gin = torch.empty_like(w_in) if dw_in is None else dw_in
+        gout = torch.empty_like(w_out) if dw_out is None else dw_out
         dgu = x.new_empty((m.rows, 2, m.inner))
         check(_lib().ugdr_x_expert_ffn_backward(m, spans["dy"][0], spans["x"][0], spans["saved.h"][0],
                                                 spans["saved.gu"][0], dgu.data_ptr(), gx.data_ptr(), gin.data_ptr(),
