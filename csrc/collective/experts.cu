@@ -434,7 +434,8 @@ __device__ __forceinline__ void add8(const float *p, float (&v)[8]) {
 
 // a(g) and a'(g).  silu's exponential and quotient are the approximate ones: together off by less
 // than (|g| + 8) 2^-23 of the value, which goes under in the rounding to 16 bits (2^-12 of it at best).
-// 1 + exp(-g) is between 1 and infinity, whose quotient is the 0 that belongs there.
+// 1 + exp(-g) is between 1 and infinity.  From 2^126 on, at g < -87.3, the quotient is 0: it is below
+// 2^-126 there, and a(g) and a'(g) below 2^-119.
 struct Act {
     float a, da;
 };

@@ -110,6 +110,24 @@ def test_ranges_where_fp32_squares_leave_their_type(scale):
         assert abs(float(GradClip(grads).clip(float("inf"))) - want) <= NORM_REL * want
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("scale", [1e-30, 1.0])
+def test_groups_of_zeros_between_others(dtype, scale):
+    """Groups of zeros of either sign between numbers whose squares fp32 holds, or does not."""
+    from ugdr_b200.ops import GradClip
+
+    dtype = getattr(torch, dtype)
+    if dtype == torch.float16 and scale < 1:
+        scale = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps  # its smallest number
+    for n in (40, 8 * 4096 + 5, 3_000_007):
+        g = torch.zeros(n, dtype=dtype, device="cuda")
+        g[torch.arange(n, device="cuda") % 48 < 16] = -0.0
+        g[::40] = scale
+        g[n // 2:n // 2 + 3] = 2 * scale
+        want = norm64([g])
+        assert want > 0 and abs(float(GradClip([g]).clip(float("inf"))) - want) <= NORM_REL * want
+
+
 def test_zeros_infinities_and_nans():
     from ugdr_b200.ops import GradClip
 
