@@ -275,10 +275,13 @@ template <Product P> __device__ __forceinline__ int steps_of(const Shape &m, int
 
 // Walks a worker's share of the tile list: one tile of every round.
 //
-// An expert's rows are cut into tiles of about the same size, all but the last a multiple of kStepN.
-// (Tiles of up to 512 rows, in both accumulators, load the features once for more rows; they gained
-// 4 % at 300 rows per expert and cost 1 to 4 % elsewhere, for the longer code and the accumulators
-// that no products run beside.)
+// An expert's rows are cut into as few tiles as kMaxN allows, of about the same size, all but the last a
+// multiple of kStepN.  Shared memory, 128 bytes per clock, sets the price of a tile of N rows: a step
+// writes 128 + N / 2 clocks' worth and its four instructions read 4 (32 + N / 8), together 256 + N,
+// beside 2 N for the products.  So N = 256 is in balance, and 32 experts of 288 rows, as 160 + 128, take
+// 1.44 times as long as of 256 (832 and 577 us, 7168 x 2048).  (Tiles of up to 512 rows, whose features
+// are loaded once and read by two instructions, gained 4 % from 264 to 320 rows and cost 3 to 6 %
+// elsewhere, for accumulators that cannot take turns as a whole.)
 //
 // A weight gradient's tiles take as long as their expert has rows, so the experts with the most rows
 // come first, and the pairs take turns forwards and backwards: over 28,813 rows of 17 uneven experts,
