@@ -54,7 +54,8 @@ class GradClip:
     The plan holds the tensors and their addresses: gradients that are replaced (not written in
     place) need a new plan.  Its methods are enqueued on `stream` (default: the device's current
     stream), may be captured into a CUDA graph, and can run on several streams at once as far as
-    the gradients allow it."""
+    the gradients allow it.  A plan may be dropped with calls still under way, on any stream, but a
+    graph that captured a call holds the plan's addresses, not the plan, which has to outlive it."""
 
     def __init__(self, grads: Sequence[torch.Tensor], out: Sequence[torch.Tensor] | None = None):
         self.grads = tuple(grads)
@@ -91,6 +92,9 @@ class GradClip:
         self._plan, self._n, self._chunks = plan.to(self.device), n, chunks.value
         # The copy is over: any stream may use the plan.
         torch.cuda.current_stream(self.device).synchronize()
+        # The allocator knows of the stream that the table was made on only; _keep tells it of others.
+        self._home = torch._C._cuda_getCurrentRawStream(self.device.index)
+        self._kept: set[int] = set()
 
     def _refuse_overlaps(self) -> None:
         """Memory that is written is written for one tensor only, and read for that one only."""
@@ -109,16 +113,27 @@ class GradClip:
             end = max(end, b)
             written = max(written, b) if writes else written
 
+    def _keep(self, s: int, chosen: bool) -> None:
+        """Keep the plan's memory from reuse until the current stream, `s`, is through with it, should
+        the plan be dropped before.  (Once per stream: the plan's own references do the rest.)"""
+        if s in self._kept or (s == self._home and not chosen):
+            return
+        stream = torch.cuda.current_stream(self.device)
+        for t in (self._plan, *self.grads, *(self.out if self.out is not self.grads else ())):
+            t.record_stream(stream)
+        self._kept.add(s)
+
     def sum_squares(self, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
         """The sum of the squares of all elements, a float64 tensor on the device."""
         def call(s):
+            self._keep(s, stream is not None)
             partials = self._plan.new_empty(PARTIALS, dtype=torch.float64)
             total = self._plan.new_empty((), dtype=torch.float64)
             check(_lib().ugdr_x_grad_sum_squares(self._plan.data_ptr(), self._n, self._chunks, partials.data_ptr(),
                                                  total.data_ptr(), s), "ugdr_x_grad_sum_squares")
             return total
 
-        return _enqueue(self.device, stream, (self._plan, *self.grads), call)
+        return _enqueue(self.device, stream, (), call)
 
     def clip(self, max_norm: float, sum_squares: torch.Tensor | None = None,
              stream: torch.cuda.Stream | None = None) -> torch.Tensor:
@@ -132,7 +147,9 @@ class GradClip:
         if sum_squares is not None and (not isinstance(sum_squares, torch.Tensor) or sum_squares.numel() != 1
                                         or sum_squares.dtype != torch.float64 or sum_squares.device != self.device):
             raise ValueError(f"sum_squares must be one float64 on {self.device}")
+
         def call(s):
+            self._keep(s, stream is not None)
             partials = self._plan.new_empty(PARTIALS, dtype=torch.float64)
             norm = self._plan.new_empty((), dtype=torch.float32)
             check(_lib().ugdr_x_grad_clip(self._plan.data_ptr(), self._n, self._chunks, partials.data_ptr(),
@@ -140,5 +157,4 @@ class GradClip:
                                           norm.data_ptr(), s), "ugdr_x_grad_clip")
             return norm
 
-        return _enqueue(self.device, stream, (self._plan, *self.grads, *self.out,
-                                              *(() if sum_squares is None else (sum_squares,))), call)
+        return _enqueue(self.device, stream, () if sum_squares is None else (sum_squares,), call)
