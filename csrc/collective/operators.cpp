@@ -65,10 +65,15 @@ int ugdr_x_grad_plan(const ugdr_x_grad *grads, int n, void *plan, uint64_t *chun
         if (g.count > 0 && (g.grad == nullptr || reinterpret_cast<uintptr_t>(g.grad) % element_bytes(g.grad_type) ||
                             g.out == nullptr || reinterpret_cast<uintptr_t>(g.out) % element_bytes(g.out_type)))
             return int(cudaErrorInvalidValue);
+        if (g.count > (uint64_t(1) << 44)) return int(cudaErrorInvalidValue);
+        // In place works element by element; elements of another size would land on ones yet to be read.
+        const auto in = reinterpret_cast<uintptr_t>(g.grad), out = reinterpret_cast<uintptr_t>(g.out);
+        if (g.count > 0 && (in != out || g.out_type != g.grad_type) && out < in + g.count * element_bytes(g.grad_type) &&
+            in < out + g.count * element_bytes(g.out_type))
+            return int(cudaErrorInvalidValue);
         // A tensor's first chunk begins before its first element, on a boundary of 8 elements.
         const size_t width = element_bytes(g.grad_type);
-        const uint64_t lead = reinterpret_cast<uintptr_t>(g.grad) % (8 * width) / width;
-        if (g.count > (uint64_t(1) << 44)) return int(cudaErrorInvalidValue);
+        const uint64_t lead = in % (8 * width) / width;
         if (g.count > 0) at += (g.count + lead + ugdr::coll::kGradChunk - 1) / ugdr::coll::kGradChunk;
         if (at > UINT32_MAX) return int(cudaErrorInvalidValue);
     }

@@ -60,9 +60,10 @@ int ugdr_x_expert_ffn(const ugdr_x_experts *m, const void *x, void *y, void *h, 
 int ugdr_x_expert_ffn_backward(const ugdr_x_experts *m, const void *dy, const void *x, const void *h, const float *gu,
                                void *dgu, void *dx, void *dw_in, void *dw_out, void *stream);
 
-/* One gradient tensor of a plan: `count` elements of `grad_type` at `grad`, scaled into `out`
- * (`grad` itself, or other memory) as elements of `out_type` (grad_type, or FP32).  Pointers are
- * aligned to their element. */
+/* One gradient tensor of a plan: `count` elements of `grad_type` at `grad`, scaled into `out` as
+ * elements of `out_type` (grad_type, or FP32).  `out` is `grad` itself, with the same type, or memory
+ * that overlaps no gradient and no other output; ugdr_x_grad_plan refuses a tensor whose `out` overlaps
+ * its own `grad` in any other way.  Pointers are aligned to their element. */
 typedef struct ugdr_x_grad {
     const void *grad;
     void *out;
