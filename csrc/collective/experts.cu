@@ -32,7 +32,7 @@
 // that the power limit leaves, with the tensor pipes 92 to 98 % busy.  One row for each of 32 experts
 // reads their 2.8 GB at 6.8 TB/s.  In between, a step takes the ring's latency, about 0.3 us.
 //
-// Every wait is bounded: one that runs out sets *status and ends the kernel.
+// Every wait is bounded (ugdr_x_set_expert_wait_ns): one that runs out sets *status and ends the kernel.
 #include "collective/operators.hpp"
 
 #include <cuda.h>
@@ -61,7 +61,6 @@ constexpr uint32_t kOperandBytes = kHalf * kDepth * 2;  // one CTA's half of A, 
 constexpr uint32_t kRingBytes = 6 * 2 * kOperandBytes;  // 6 stages for the largest N, 10 for the smallest
 constexpr int kStagingRow = kHalf + 4;                  // floats; the 4 keep 16-byte reads apart
 constexpr uint32_t kStagingBytes = kChunk * kStagingRow * 4;
-constexpr uint64_t kWaitNs = 5ull * 1000 * 1000 * 1000;
 
 enum Product { kUp, kDown, kBack, kInput, kGradOut, kGradIn };
 template <Product P> constexpr bool kWeightGrad = P == kGradOut || P == kGradIn;
@@ -71,6 +70,7 @@ template <Product P> constexpr bool kFeaturesInner = P != kUp && P != kDown;
 struct Shape {
     const int32_t *counts;
     unsigned int *status;
+    uint64_t wait_ns;  // bound of every wait
     int rows, nexp, hidden, inner, act;
     int stages;            // of the ring, and the bytes of one: B's part is what the rows can need
     uint32_t stage_bytes;
@@ -140,16 +140,16 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
 }
 // Waits until the barrier's phase of `parity` is over.  False: the wait, or another of this CTA,
 // ran out, and the caller gives up.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, Shared &sh, unsigned int *status) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, Shared &sh, const Shape &m) {
     uint64_t since = 0;
     for (uint32_t spins = 1; !mbar_try(bar, parity); ++spins) {
         if (spins % 64 != 0) continue;
         if (*reinterpret_cast<volatile int *>(&sh.aborted)) return false;
         const uint64_t now = gtime();
         if (since == 0) since = now;
-        if (now - since > kWaitNs) {
+        if (now - since > m.wait_ns) {
             *reinterpret_cast<volatile int *>(&sh.aborted) = 1;
-            atomicExch(status, 1u);
+            atomicExch(m.status, 1u);
             return false;
         }
     }
@@ -485,7 +485,7 @@ template <Product P> struct Loader {
     Ring at;
     bool started = false;
 
-    __device__ __forceinline__ bool wait() { return mbar_wait(empty + at.bar, at.parity, sh, m.status); }
+    __device__ __forceinline__ bool wait() { return mbar_wait(empty + at.bar, at.parity, sh, m); }
 
     // Steps [k0, k1) of a tile.
     __device__ __forceinline__ bool load_tile(const Tile &t, int k0, int k1) {
@@ -602,7 +602,7 @@ template <typename T, Product P> struct Issuer {
     Ring at;
 
     __device__ __forceinline__ bool wait() {
-        if (!mbar_wait(full + at.bar, at.parity, sh, m.status)) return false;
+        if (!mbar_wait(full + at.bar, at.parity, sh, m)) return false;
         fence_after();
         return true;
     }
@@ -733,6 +733,7 @@ __device__ __forceinline__ void tear_down(const Setup &k) {
     __syncthreads();
     if (k.sh->aborted) {  // loads and instructions that are still under way end within this time
         for (const uint64_t since = gtime(); gtime() - since < 2'000'000;) __nanosleep(1000);
+        __syncwarp();
     }
     fence_before();
     cluster_sync();
@@ -773,7 +774,7 @@ struct TailClearer {
         it += uint32_t(k1 - k0);
         if (k1 == k0 || last == 0 || k1 * kDepth < rows) return true;
         const uint32_t s = (it - 1) % uint32_t(m.stages);
-        if (!mbar_wait(smem_addr(&sh.tail[s]), phases >> s & 1, sh, m.status)) return false;
+        if (!mbar_wait(smem_addr(&sh.tail[s]), phases >> s & 1, sh, m)) return false;
         phases ^= 1u << s;
         uint8_t *stage = k.ring + s * m.stage_bytes;
         const int count = ceil_div(last, 16) * 16 - last;  // rows of 128 bytes, in each of 4 tiles
@@ -810,7 +811,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         while (tiles.next(t)) {
             const int steps = steps_of<P>(m, t.rows);
             if (steps == 0) continue;
-            if (!mbar_wait(smem_addr(&sh.tmem_empty[acc & 1]), (acc / 2 + 1) & 1, sh, m.status)) break;
+            if (!mbar_wait(smem_addr(&sh.tmem_empty[acc & 1]), (acc / 2 + 1) & 1, sh, m)) break;
             fence_after();
             if (!issuer.run(t, sh.tmem + (acc & 1) * kMaxN, 0, steps)) break;
             mma_commit(smem_addr(&sh.tmem_full[acc & 1]), issuer.mask);
@@ -829,7 +830,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const bool none = steps_of<P>(m, t.rows) == 0;
             const int feature = t.feature + int(k.rank) * (kTileFeatures<P> / 2);
             if (!none) {
-                if (!group_all(group, mbar_wait(smem_addr(&sh.tmem_full[acc & 1]), (acc / 2) & 1, sh, m.status)))
+                if (!group_all(group, mbar_wait(smem_addr(&sh.tmem_full[acc & 1]), (acc / 2) & 1, sh, m)))
                     break;
                 fence_after();
             }
@@ -922,7 +923,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // add their sums up through distributed shared memory, in the pairs' order.  A tile's K loop runs at
 // the latency of its ring, so one pair reads weights at a few hundred GB/s however idle the GPU is:
 // a [1, 5632] x [5632, 2048] product has 8 tiles, and took 27.9 us with a pair each, 13.1 with four.
-// Likewise dw_out of 25,409 rows of one expert, 144 x 2440, with 10 tiles: 131 and 50 us.
+// Likewise dw_out of 25,409 rows of one expert, 144 x 2440, with 10 tiles: 131 and 50 us.  There are as
+// many clusters as tiles at least (split_of), so a cluster has one tile or none.
 template <typename T, Product P>
 __global__ void __launch_bounds__(kThreads, 1)
     expert_split_kernel(const __grid_constant__ Maps maps, const Shape m, T *out, float *gu) {
@@ -933,32 +935,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int cluster = int(blockIdx.x) / (2 * split), clusters = int(gridDim.x) / (2 * split);
     Tiles<P> tiles(m, k.first, sh.order, cluster, clusters);
     Tile t;
-    Loader<P> loader = loader_of<P>(maps, m, k);
-    Issuer<T, P> issuer = issuer_of<T, P>(m, k);
-    TailClearer clearer{m, sh, k};
-    uint32_t phase = 0;
-
-    for (bool begun = false; tiles.next(t); begun = true) {
+    if (tiles.next(t)) {
         const int steps = steps_of<P>(m, t.rows), k0 = steps * part / split, k1 = steps * (part + 1) / split;
         const int n = kWeightGrad<P> ? kMaxN : ceil_div(t.rows, kStepN) * kStepN, columns = n / split;  // each pair's
         const int feature = t.feature + int(k.rank) * (kTileFeatures<P> / 2);
         if (warp == 0 && lane == 0) {
-            loader.load_tile(t, k0, k1);
+            loader_of<P>(maps, m, k).load_tile(t, k0, k1);
         } else if (warp == 1 && lane == 0 && k.rank == 0) {
+            Issuer<T, P> issuer = issuer_of<T, P>(m, k);
             if (k1 > k0 && issuer.run(t, sh.tmem, k0, k1)) mma_commit(smem_addr(&sh.tmem_full[0]), issuer.mask);
         } else if (warp == 2 && kWeightGrad<P>) {
-            clearer.clear(t.rows, k0, k1);
+            TailClearer{m, sh, k}.clear(t.rows, k0, k1);
         } else if (warp >= 4 && k1 > k0) {
-            mbar_wait(smem_addr(&sh.tmem_full[0]), phase, sh, m.status);
+            mbar_wait(smem_addr(&sh.tmem_full[0]), 0, sh, m);
         }
-        phase ^= uint32_t(k1 > k0);
         __syncthreads();
-        const bool fine = !sh.aborted;
+        const bool fine = !sh.aborted;  // else the waits ran out: nothing is stored
         // The sums, [part][column][feature], go where the epilogue's staging is, or, if that is too
         // small, into the ring, once every pair's products are over and no load is under way.
         const bool apart = n * kStagingRow * 4 <= int(2 * kStagingBytes);
         float *sums = apart ? k.staging : reinterpret_cast<float *>(k.ring);
-        if (begun || !apart) cluster_sync();
+        if (!apart) cluster_sync();
         fence_after();
         if (fine && warp >= 4 && k1 > k0) {
             const int quarter = warp % 4, group = warp / 4 - 1;
@@ -1008,9 +1005,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 finish<T, P>(m, out, gu, row, f, a, b, g, u);
             }
         }
-        // The ring is the loads' again.
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncthreads();
     }
     if (threadIdx.x == 0) wait_previous();
     tear_down(k);
@@ -1095,7 +1089,7 @@ cudaError_t residency(const void *kernel, bool split, int device, int index, Res
     return cudaSuccess;
 }
 
-// Pairs that share a tile: as many as let every tile have a cluster on the GPU at once, where the steps
+// Pairs that share a tile: as many as let every tile have a cluster of the launch, where the steps
 // are enough to gain by it.  What counts is known here from above only: a tile for each expert, or row
 // if those are fewer, and one for every kMaxN rows; for the weight gradients, whose steps are an
 // expert's rows, their mean.
@@ -1152,7 +1146,7 @@ cudaError_t launch(const ugdr_x_experts &m, const void *a, const void *b, void *
         db.box[db.rank - 1] = kWeightGrad<P> ? kDepth : kHalf >> i;
         if (!encode<T>(&maps.b[i], db)) return cudaErrorInvalidValue;
     }
-    const Shape shape{m.counts, m.status, int(m.rows), m.nexp, m.hidden, m.inner, m.act, stages, stage_bytes};
+    const Shape shape{m.counts, m.status, expert_wait_ns(), int(m.rows), m.nexp, m.hidden, m.inner, m.act, stages, stage_bytes};
 
     int device = 0;
     if (cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return e;

@@ -1,9 +1,13 @@
 // C ABI of the model operators: argument checks, then the launches of experts.cu and grad_clip.cu.
 #include "collective/operators.hpp"
 
+#include <atomic>
 #include <cstring>
 
 namespace {
+
+constexpr uint64_t kDefaultWaitNs = 5ull * 1000 * 1000 * 1000;
+std::atomic<uint64_t> g_wait_ns{kDefaultWaitNs};
 
 bool aligned16(const void *p) { return p != nullptr && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 bool aligned32(const void *p) { return p != nullptr && reinterpret_cast<uintptr_t>(p) % 32 == 0; }
@@ -21,7 +25,11 @@ size_t element_bytes(int type) { return type == UGDR_X_TYPE_FP32 ? 4 : 2; }
 
 }  // namespace
 
+uint64_t ugdr::coll::expert_wait_ns() { return g_wait_ns.load(std::memory_order_relaxed); }
+
 extern "C" {
+
+uint64_t ugdr_x_set_expert_wait_ns(uint64_t ns) { return g_wait_ns.exchange(ns == 0 ? kDefaultWaitNs : ns); }
 
 int ugdr_x_expert_ffn(const ugdr_x_experts *m, const void *x, void *y, void *h, float *gu, void *stream) {
     if (!valid(m)) return int(cudaErrorInvalidValue);

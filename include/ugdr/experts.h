@@ -48,6 +48,11 @@ typedef struct ugdr_x_experts {
     int act;
 } ugdr_x_experts;
 
+/* Bound, in ns, of every wait inside the kernels of the calls below that are launched from now on (0: the
+ * default, 5 s).  Returns the one before.  A wait takes as long as the longest tile of a product, so a
+ * bound of less than some milliseconds can run out in calls that are fine. */
+uint64_t ugdr_x_set_expert_wait_ns(uint64_t ns);
+
 /* Forward: g = x Wg^T, u = x Wu^T, h = a(g) * u, y = h Wo^T.  `h` ([rows][inner]) is scratch of a
  * serving call; with `gu` ([rows][2][inner] floats on a 32-byte boundary, may be NULL) g and u are kept
  * too, and h and gu are what the backward pass takes.  y may be x itself (the products with x are over by then). */
