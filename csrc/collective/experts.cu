@@ -446,9 +446,25 @@ __device__ __forceinline__ Act silu(float g) {
     const float s = __fdividef(1.f, 1.f + __expf(-g));
     return {g * s, s * (1.f + g * (1.f - s))};
 }
+// gelu: g Phi(g), with Phi(-|g|) = exp(-g^2 / 2) t q(t), t = 1 / (1 + 0.3 |g|), so that the lower tail keeps
+// its relative precision, which 1 + erf does not (off by 4 % at g = -5, and 0 from -5.5 on).  q is a least
+// squares fit, reweighted towards the smallest largest relative error (1.5e-7), to
+// exp(g^2 / 2) Phi(-|g|) / t at 2000 Chebyshev nodes over |g| <= 14.  With the approximate exponential,
+// which the derivative needs too, and quotient, Phi is off by less than (g^2 + 12) 2^-23 of its value, down
+// to g = -13, where it leaves fp32's normal numbers.
 __device__ __forceinline__ Act gelu(float g) {
-    const float p = 0.5f + 0.5f * erff(g * 0.70710678f);
-    return {g * p, p + g * 0.39894228f * expf(-0.5f * g * g)};
+    const float t = __fdividef(1.f, 1.f + 0.3f * fabsf(g)), e = __expf(-0.5f * g * g);
+    float q = 0.0356748775f;
+    q = fmaf(q, t, -0.157203496f);
+    q = fmaf(q, t, 0.206354201f);
+    q = fmaf(q, t, -0.0536842458f);
+    q = fmaf(q, t, 0.128561929f);
+    q = fmaf(q, t, 0.0999134108f);
+    q = fmaf(q, t, 0.120753966f);
+    q = fmaf(q, t, 0.119629301f);
+    q *= t * e;
+    const float p = g > 0.f ? 1.f - q : q;
+    return {g * p, p + g * 0.39894228f * e};
 }
 
 // ---- the kernel --------------------------------------------------------------------------------
