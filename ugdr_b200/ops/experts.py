@@ -92,7 +92,8 @@ def _status_word(device: torch.device) -> torch.Tensor:
     if word is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("call an expert operator once on this device before capturing it into a graph")
-        word = torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # else only inference mode could clear it
+            word = torch.zeros(1, dtype=torch.int32, device=device)
         torch.cuda.current_stream(device).synchronize()  # zero before any stream may write it
         word = _status.setdefault(device.index, word)
     return word
