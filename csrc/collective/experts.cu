@@ -47,6 +47,7 @@ namespace ugdr::coll {
 namespace {
 
 constexpr int kThreads = 384;       // 12 warps: 4 that feed the tensor cores, 8 for the epilogue
+constexpr int kCheckThreads = 256;
 constexpr int kHalf = 128;          // features of a tile per CTA: the lanes of TMEM
 constexpr int kPairFeatures = 256;
 constexpr int kMaxN = 256;
@@ -1026,6 +1027,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     tear_down(k);
 }
 
+// A call without rows has nothing to do but to look for counts that say otherwise.
+__global__ void count_check_kernel(const int32_t *counts, int nexp, unsigned int *status) {
+    int any = 0;
+    for (int e = threadIdx.x; e < nexp; e += blockDim.x) any |= counts[e];
+    if (__syncthreads_or(any) && threadIdx.x == 0) atomicExch(status, 2u);
+}
+
 // ---- launches ----------------------------------------------------------------------------------
 
 using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
@@ -1224,9 +1232,15 @@ int backward(const ugdr_x_experts &m, const void *dy, const void *x, const void 
 int expert_kernels(const KernelRef **out) {
     static const KernelRef refs[] = {
         UGDR_EXPERT_ALL(expert_kernel, __nv_bfloat16, "bf16"), UGDR_EXPERT_ALL(expert_kernel, __half, "fp16"),
-        UGDR_EXPERT_ALL(expert_split_kernel, __nv_bfloat16, "bf16"), UGDR_EXPERT_ALL(expert_split_kernel, __half, "fp16")};
+        UGDR_EXPERT_ALL(expert_split_kernel, __nv_bfloat16, "bf16"), UGDR_EXPERT_ALL(expert_split_kernel, __half, "fp16"),
+        {"count_check_kernel", reinterpret_cast<const void *>(&count_check_kernel), kCheckThreads}};
     *out = refs;
     return int(sizeof(refs) / sizeof(refs[0]));
+}
+
+int launch_count_check(const ugdr_x_experts &m, cudaStream_t s) {
+    count_check_kernel<<<1, kCheckThreads, 0, s>>>(m.counts, m.nexp, m.status);
+    return int(cudaGetLastError());
 }
 
 int launch_expert_ffn(const ugdr_x_experts &m, const void *x, void *y, void *h, float *gu, cudaStream_t s) {

@@ -33,7 +33,7 @@ uint64_t ugdr_x_set_expert_wait_ns(uint64_t ns) { return g_wait_ns.exchange(ns =
 
 int ugdr_x_expert_ffn(const ugdr_x_experts *m, const void *x, void *y, void *h, float *gu, void *stream) {
     if (!valid(m)) return int(cudaErrorInvalidValue);
-    if (m->rows == 0) return int(cudaSuccess);
+    if (m->rows == 0) return ugdr::coll::launch_count_check(*m, static_cast<cudaStream_t>(stream));
     if (!aligned16(x) || !aligned16(y) || !aligned16(h) || (gu != nullptr && !aligned32(gu)))
         return int(cudaErrorInvalidValue);
     return ugdr::coll::launch_expert_ffn(*m, x, y, h, gu, static_cast<cudaStream_t>(stream));
@@ -46,7 +46,8 @@ int ugdr_x_expert_ffn_backward(const ugdr_x_experts *m, const void *dy, const vo
     if (m->rows == 0) {
         const size_t block = size_t(m->nexp) * size_t(m->inner) * size_t(m->hidden) * 2;
         if (const cudaError_t e = cudaMemsetAsync(dw_in, 0, 2 * block, s); e != cudaSuccess) return int(e);
-        return int(cudaMemsetAsync(dw_out, 0, block, s));
+        if (const cudaError_t e = cudaMemsetAsync(dw_out, 0, block, s); e != cudaSuccess) return int(e);
+        return ugdr::coll::launch_count_check(*m, s);
     }
     if (!aligned16(dy) || !aligned16(x) || !aligned16(h) || !aligned32(gu) || !aligned16(dgu) || !aligned16(dx))
         return int(cudaErrorInvalidValue);

@@ -11,6 +11,7 @@
 namespace ugdr::coll {
 
 uint64_t expert_wait_ns();  // bound of the waits in the experts' kernels
+int launch_count_check(const ugdr_x_experts &m, cudaStream_t s);  // for calls without rows
 int launch_expert_ffn(const ugdr_x_experts &m, const void *x, void *y, void *h, float *gu, cudaStream_t s);
 int launch_expert_ffn_backward(const ugdr_x_experts &m, const void *dy, const void *x, const void *h, const float *gu,
                                void *dgu, void *dx, void *dw_in, void *dw_out, cudaStream_t s);
