@@ -258,6 +258,20 @@ __global__ void __launch_bounds__(kThreads) grad_sum_kernel(const double *partia
     if (threadIdx.x == 0) *sum_squares = s;
 }
 
+// The chunks [c0, c1) of one tensor scaled into an output whose whole groups are not aligned: neighbours to
+// neighbouring threads.  Out of line, since the other path's registers spilled beside it.
+template <typename T, typename O>
+__device__ __noinline__ void span_scale_apart(const T *g, O *out, int64_t n, uint32_t lead, uint32_t c0, uint32_t c1,
+                                              float coef) {
+    for (uint32_t c = c0; c < c1; ++c) {
+        const int64_t at = int64_t(c) * kGradChunk - int64_t(lead) + threadIdx.x;
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j)
+            if (at + j * kThreads >= 0 && at + j * kThreads < n)
+                from_float(out[at + j * kThreads], to_float(g[at + j * kThreads]) * coef);
+    }
+}
+
 // The chunks [c0, c1) of one tensor scaled, the last ones first.
 template <int IN, int OUT> __device__ void span_scale(const ugdr_x_grad &t, uint32_t c0, uint32_t c1, float coef) {
     using T = typename Element<IN>::type;
@@ -268,15 +282,7 @@ template <int IN, int OUT> __device__ void span_scale(const ugdr_x_grad &t, uint
     const uint32_t lead = lead_of(g);
     const int64_t n = int64_t(t.count);
     const auto one = [&](int64_t i) { from_float(out[i], to_float(g[i]) * coef); };
-    if (lead_of(out) != lead) {  // whole groups of the output are not aligned: neighbours to neighbouring threads
-        for (uint32_t c = c0; c < c1; ++c) {
-            const int64_t at = int64_t(c) * kGradChunk - int64_t(lead) + threadIdx.x;
-#pragma unroll
-            for (int j = 0; j < kGroup; ++j)
-                if (at + j * kThreads >= 0 && at + j * kThreads < n) one(at + j * kThreads);
-        }
-        return;
-    }
+    if (lead_of(out) != lead) return span_scale_apart(g, out, n, lead, c0, c1, coef);
     const Mine w = my_chunks(c0, c1, lead, n);
     const int64_t begin = int64_t(w.b) * kGradChunk + threadIdx.x * kGroup - int64_t(lead);
     const T *p = g + begin;
