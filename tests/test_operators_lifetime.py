@@ -40,7 +40,7 @@ def plan(monkeypatch):
     p = grads.GradClip.__new__(grads.GradClip)
     p.device, p.grads, p._plan, p._n, p._chunks = torch.device("cuda", 0), (Block(), Block()), Block(), 2, 2
     p.out = (p.grads[0], Block())
-    p._home, p._kept = 7, set()
+    p._home, p._kept, p._written = 7, set(), ()
     return p, lambda s: at.__setitem__(0, s)
 
 

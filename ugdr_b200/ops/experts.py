@@ -24,7 +24,7 @@ them, as it does when a bounded wait inside a kernel ran out.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Iterable, NamedTuple
+from typing import Iterable, NamedTuple, Sequence
 
 import torch
 
@@ -69,21 +69,27 @@ def _lib() -> C.CDLL:
     return _bound
 
 
-def _enqueue(device: torch.device, stream: torch.cuda.Stream | None, tensors: Iterable[torch.Tensor], call):
+def _enqueue(device: torch.device, stream: torch.cuda.Stream | None, tensors: Iterable[torch.Tensor], call,
+             written: Sequence[torch.Tensor] = ()):
     """call(raw stream) with the tensors' device current and `stream` (default: the device's current
     one) the stream that outputs and scratch are allocated for.  On a stream of the caller's choice the
-    tensors' memory is kept from reuse until the stream is through with it."""
+    tensors' memory is kept from reuse until the stream is through with it.  Those that are `written`
+    get new versions, so that a backward pass which saved one of them raises torch's error."""
     if stream is None:
         if torch.cuda.current_device() == device.index:  # the short way
-            return call(torch._C._cuda_getCurrentRawStream(device.index))
-        with torch.cuda.device(device):
-            return call(torch._C._cuda_getCurrentRawStream(device.index))
-    if stream.device != device:
-        raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
-    with torch.cuda.device(device), torch.cuda.stream(stream):
-        result = call(stream.cuda_stream)
-    for t in tensors:
-        t.record_stream(stream)
+            result = call(torch._C._cuda_getCurrentRawStream(device.index))
+        else:
+            with torch.cuda.device(device):
+                result = call(torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        if stream.device != device:
+            raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+        with torch.cuda.device(device), torch.cuda.stream(stream):
+            result = call(stream.cuda_stream)
+        for t in tensors:
+            t.record_stream(stream)
+    if written:
+        torch.autograd.graph.increment_version(written)
     return result
 
 
@@ -179,7 +185,8 @@ def _forward(x, counts, w_in, w_out, act, out, stream, train):
                                        s), "ugdr_x_expert_ffn")
         return y, ExpertFFNSaved(h, gu) if train else None
 
-    return _enqueue(x.device, stream, (x, counts, w_in, w_out) if out is None else (x, counts, w_in, w_out, out), call)
+    given = () if out is None else (out,)
+    return _enqueue(x.device, stream, (x, counts, w_in, w_out, *given), call, given)
 
 
 def expert_ffn(x: torch.Tensor, counts: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, act: str = "silu",
@@ -212,13 +219,13 @@ def expert_ffn_backward(dy: torch.Tensor, x: torch.Tensor, counts: torch.Tensor,
     spans["saved.gu"] = _span(saved.gu, "saved.gu", (m.rows, 2, m.inner), torch.float32, device)
     if spans["saved.gu"][0] % 32:
         raise ValueError("saved.gu must be 32-byte aligned")
-    tensors = [x, counts, w_in, w_out, dy, saved.h, saved.gu]
+    tensors, given = [x, counts, w_in, w_out, dy, saved.h, saved.gu], []
     for name, t, shape in (("dx", dx, x.shape), ("dw_in", dw_in, w_in.shape), ("dw_out", dw_out, w_out.shape)):
         if t is not None:
             span = _span(t, name, shape, dtype, device)
             _apart(name, span, spans, ("dy", "x") if name == "dx" else ())
             spans[name] = span
-            tensors.append(t)
+            given.append(t)
 
     def call(s):
         m.status = _status_word(device).data_ptr()
@@ -231,4 +238,4 @@ def expert_ffn_backward(dy: torch.Tensor, x: torch.Tensor, counts: torch.Tensor,
                                                 gout.data_ptr(), s), "ugdr_x_expert_ffn_backward")
         return gx, gin, gout
 
-    return _enqueue(device, stream, tensors, call)
+    return _enqueue(device, stream, tensors + given, call, given)

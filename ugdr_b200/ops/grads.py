@@ -95,6 +95,9 @@ class GradClip:
         # The allocator knows of the stream that the table was made on only; _keep tells it of others.
         self._home = torch._C._cuda_getCurrentRawStream(self.device.index)
         self._kept: set[int] = set()
+        # Views share their base's version: one of each is enough.
+        bases = (o if o._base is None else o._base for o in self.out)
+        self._written = tuple({id(b): b for b in bases}.values())
 
     def _refuse_overlaps(self) -> None:
         """Memory that is written is written for one tensor only, and read for that one only."""
@@ -157,4 +160,4 @@ class GradClip:
                                           norm.data_ptr(), s), "ugdr_x_grad_clip")
             return norm
 
-        return _enqueue(self.device, stream, () if sum_squares is None else (sum_squares,), call)
+        return _enqueue(self.device, stream, () if sum_squares is None else (sum_squares,), call, self._written)
