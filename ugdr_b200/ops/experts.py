@@ -17,7 +17,9 @@ must stay within its range, as x and y must):
 
 Rows behind the last group (the unused end of a receive area) are left as they were.  Calls are
 enqueued on `stream` (default: the device's current stream), whose order the inputs must respect,
-and may be captured into a CUDA graph.  They do not take part in autograd.  Counts that are
+and may be captured into a CUDA graph.  They do not take part in autograd: `expert_ffn` refuses tensors
+whose gradients it would drop, and the training calls leave the gradients to the caller and
+`expert_ffn_backward`.  Counts that are
 negative or add up to more than `rows` are recorded on the device: `check_status()` raises for
 them, as it does when a bounded wait inside a kernel ran out.
 """
@@ -192,7 +194,13 @@ def _forward(x, counts, w_in, w_out, act, out, stream, train):
 def expert_ffn(x: torch.Tensor, counts: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, act: str = "silu",
                out: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """y [rows, hidden] of the block, into `out` if given (which may be `x` itself: the experts in
-    place in the receive area).  act: "silu" or "gelu" (the exact one)."""
+    place in the receive area).  act: "silu" or "gelu" (the exact one).  For serving: where gradients are
+    recorded (not under torch.no_grad() or inference_mode()), no tensor may require one."""
+    if torch.is_grad_enabled():
+        for name, t in (("x", x), ("w_in", w_in), ("w_out", w_out), ("out", out)):
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                raise ValueError(f"{name} requires a gradient, which expert_ffn does not record: call it under "
+                                 "torch.no_grad(), or use expert_ffn_train and expert_ffn_backward")
     return _forward(x, counts, w_in, w_out, act, out, stream, False)[0]
 
 
