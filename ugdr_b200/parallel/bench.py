@@ -15,7 +15,8 @@
   torch kernels and the split sizes exchanged first.  With --inner F the step is also timed with
   real experts, gated feed-forward blocks of inner size F, between dispatch and combine.
 Times are CUDA-event durations of K back-to-back iterations on each rank, max over ranks.  The
-first ugdr call is checked against a torch fp32 reference.
+first ugdr call is checked against a torch fp32 reference ("correct"; with experts, a few tokens of
+every rank: "experts_correct").
 """
 from __future__ import annotations
 
@@ -249,7 +250,28 @@ def bench_p2p_nccl(rank, world, sizes, iters, warmup) -> list[dict]:
     return out
 
 
-def _moe_experts(rank, world, iters, warmup, cfg: MoEConfig, inner, g, a2a, x, ids, w) -> dict:
+def _experts_right(rank, exchange, x, ids, w, w_in, w_out, out, sample: int = 4) -> bool:
+    """Whether the MoE layer's output is right for each rank's first few tokens: every rank takes its own
+    experts' part of all of them in fp32, and each adds up its tokens'.  Off, as a token's vector, by less
+    than three roundings to bf16 (of h, of an expert's result and of their sum) and a little for fp32."""
+    sent = exchange((x[:sample].cpu(), ids[:sample].cpu()))
+    first, mine = rank * w_in.shape[0], w_in.shape[0]
+    parts = []  # of every rank's tokens: [(t, k), hidden], zeros where the expert is another rank's
+    for xs, es in sent:
+        rows, flat = xs.to(x.device).float().repeat_interleave(es.shape[1], 0), es.reshape(-1).long() - first
+        part = torch.zeros_like(rows)
+        for i, e in enumerate(flat.tolist()):
+            if 0 <= e < mine:
+                gate, up = w_in[e].float() @ rows[i]
+                part[i] = w_out[e].float() @ (torch.nn.functional.silu(gate) * up)
+        parts.append(part.cpu())
+    ref = sum(p[rank] for p in exchange(parts)).view(-1, w.shape[1], x.shape[1])
+    ref = (ref * w[:sample].float().cpu()[..., None]).sum(1)
+    off = (out[:sample].float().cpu() - ref).norm(dim=1)
+    return bool((off <= 3.5 * 2.0 ** -8 * ref.norm(dim=1)).all())
+
+
+def _moe_experts(rank, world, iters, warmup, cfg: MoEConfig, inner, exchange, g, a2a, x, ids, w) -> dict:
     """dispatch, this rank's experts in place in the receive area, combine."""
     from .. import ops
 
@@ -266,13 +288,16 @@ def _moe_experts(rank, world, iters, warmup, cfg: MoEConfig, inner, g, a2a, x, i
         a2a.ready()
         return a2a.combine(w)
 
+    out = step()
+    torch.cuda.synchronize()
+    right = all(exchange(_experts_right(rank, exchange, x, ids, w, w_in, w_out, out)))
     t = _timed(step, iters, warmup)
     g.check_status()
     ops.check_status()
     rows = torch.tensor([float(a2a.recv_used.item())], dtype=torch.float64)
     dist.all_reduce(rows, group=_GLOO)
     return {"inner": inner, "ugdr_with_experts_ms": round(t, 4),
-            "experts_TFLOPs_per_gpu": round(6 * float(rows) * H * inner / world / t / 1e9, 1)}
+            "experts_TFLOPs_per_gpu": round(6 * float(rows) * H * inner / world / t / 1e9, 1), "experts_correct": right}
 
 
 def bench_moe(rank, world, iters, warmup, cfg: MoEConfig, inner: int = 0) -> dict:
@@ -302,7 +327,7 @@ def bench_moe(rank, world, iters, warmup, cfg: MoEConfig, inner: int = 0) -> dic
     t_ugdr = _timed(ugdr_step, iters, warmup)
     g.check_status()
 
-    experts = _moe_experts(rank, world, iters, warmup, cfg, inner, g, a2a, x, ids, w) if inner else {}
+    experts = _moe_experts(rank, world, iters, warmup, cfg, inner, exchange, g, a2a, x, ids, w) if inner else {}
 
     # NCCL baseline: permute by destination rank, exchange split sizes, all_to_all_single,
     # (identity experts), reverse all_to_all_single, weighted un-permute.
