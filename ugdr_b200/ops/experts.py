@@ -53,6 +53,7 @@ class ExpertFFNSaved(NamedTuple):
     gu: torch.Tensor  # [rows, 2, inner] float32: both projections
 
 
+_new_versions = torch.autograd.graph.increment_version
 _status: dict[int, torch.Tensor] = {}
 
 
@@ -71,8 +72,8 @@ def _lib() -> C.CDLL:
     return _bound
 
 
-def _enqueue(device: torch.device, stream: torch.cuda.Stream | None, tensors: Iterable[torch.Tensor], call,
-             written: Sequence[torch.Tensor] = ()):
+def _enqueue(device: torch.device, stream: torch.cuda.Stream | None, read: Iterable[torch.Tensor],
+             written: Sequence[torch.Tensor], call):
     """call(raw stream) with the tensors' device current and `stream` (default: the device's current
     one) the stream that outputs and scratch are allocated for.  On a stream of the caller's choice the
     tensors' memory is kept from reuse until the stream is through with it.  Those that are `written`
@@ -88,10 +89,10 @@ def _enqueue(device: torch.device, stream: torch.cuda.Stream | None, tensors: It
             raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
         with torch.cuda.device(device), torch.cuda.stream(stream):
             result = call(stream.cuda_stream)
-        for t in tensors:
+        for t in (*read, *written):
             t.record_stream(stream)
     if written:
-        torch.autograd.graph.increment_version(written)
+        _new_versions(written)
     return result
 
 
@@ -187,8 +188,7 @@ def _forward(x, counts, w_in, w_out, act, out, stream, train):
                                        s), "ugdr_x_expert_ffn")
         return y, ExpertFFNSaved(h, gu) if train else None
 
-    given = () if out is None else (out,)
-    return _enqueue(x.device, stream, (x, counts, w_in, w_out, *given), call, given)
+    return _enqueue(x.device, stream, (x, counts, w_in, w_out), () if out is None else (out,), call)
 
 
 def expert_ffn(x: torch.Tensor, counts: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, act: str = "silu",
@@ -227,7 +227,7 @@ def expert_ffn_backward(dy: torch.Tensor, x: torch.Tensor, counts: torch.Tensor,
     spans["saved.gu"] = _span(saved.gu, "saved.gu", (m.rows, 2, m.inner), torch.float32, device)
     if spans["saved.gu"][0] % 32:
         raise ValueError("saved.gu must be 32-byte aligned")
-    tensors, given = [x, counts, w_in, w_out, dy, saved.h, saved.gu], []
+    given = []
     for name, t, shape in (("dx", dx, x.shape), ("dw_in", dw_in, w_in.shape), ("dw_out", dw_out, w_out.shape)):
         if t is not None:
             span = _span(t, name, shape, dtype, device)
@@ -246,4 +246,4 @@ def expert_ffn_backward(dy: torch.Tensor, x: torch.Tensor, counts: torch.Tensor,
                                                 gout.data_ptr(), s), "ugdr_x_expert_ffn_backward")
         return gx, gin, gout
 
-    return _enqueue(device, stream, tensors + given, call, given)
+    return _enqueue(device, stream, (x, counts, w_in, w_out, dy, *saved), given, call)

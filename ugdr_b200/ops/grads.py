@@ -15,7 +15,7 @@ import torch
 
 from .. import _native as N
 from ..parallel.peers import check
-from .experts import _enqueue
+from .experts import _enqueue, _new_versions
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 PARTIALS = 2048
@@ -136,7 +136,7 @@ class GradClip:
                                                  total.data_ptr(), s), "ugdr_x_grad_sum_squares")
             return total
 
-        return _enqueue(self.device, stream, (), call)
+        return _enqueue(self.device, stream, (), (), call)
 
     def clip(self, max_norm: float, sum_squares: torch.Tensor | None = None,
              stream: torch.cuda.Stream | None = None) -> torch.Tensor:
@@ -160,4 +160,6 @@ class GradClip:
                                           norm.data_ptr(), s), "ugdr_x_grad_clip")
             return norm
 
-        return _enqueue(self.device, stream, () if sum_squares is None else (sum_squares,), call, self._written)
+        norm = _enqueue(self.device, stream, () if sum_squares is None else (sum_squares,), (), call)
+        _new_versions(self._written)
+        return norm
