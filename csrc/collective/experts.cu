@@ -27,10 +27,11 @@
 // product.  The projections g and u that the backward pass reads are kept in fp32: in 16 bits they
 // made dx and dw_in 1.8 times as far off as one rounding of the result does, against 1.4 times now.
 //
-// Measured on a B200, 8 experts of 2,048 rows, 7168 x 2048, bf16: the six products take 622, 303
-// (y), 319, 316 (dw_out), 622 (dw_in) and 606 us (dx), 1.51 to 1.59 PFLOP/s at the 1.40 to 1.46 GHz
-// that the power limit leaves, with the tensor pipes 92 to 98 % busy.  One row for each of 32 experts
-// reads their 2.8 GB at 6.8 TB/s.  In between, a step takes the ring's latency, about 0.3 us.
+// Measured on a B200, 8 experts of 2,048 rows, 7168 x 2048, bf16: the six products take 638, 305
+// (y), 324, 317 (dw_out), 633 (dw_in) and 618 us (dx), 1.49 to 1.58 PFLOP/s at the 1.37 to 1.45 GHz
+// that the power limit leaves, with the tensor pipes 87 to 93 % busy over the whole of the kernels.  One
+// row for each of 32 experts reads their 2.8 GB at 6.8 TB/s.  In between, a step takes the ring's
+// latency, 0.26 us with few rows and 0.29 us with 256.
 //
 // Every wait is bounded (ugdr_x_set_expert_wait_ns): one that runs out sets *status and ends the kernel.
 #include "collective/operators.hpp"
@@ -1128,7 +1129,7 @@ template <Product P> int split_of(const ugdr_x_experts &m, const Residency &on) 
         tiles *= (m.rows < uint64_t(m.nexp) ? int64_t(m.rows) : m.nexp) + int64_t(m.rows / kMaxN);
         depth = P == kDown ? m.inner : P == kInput ? 2 * int64_t(m.inner) : m.hidden;
     }
-    // Adding the parts up takes 2 to 3 us, a step 0.2 us.
+    // Adding the parts up takes 2 to 3 us, a step 0.26 to 0.29 us: 15 of 20 saved, or 14 of 28, gain by it.
     if (tiles <= on.clusters8 && depth >= 20 * kDepth) return 4;
     return tiles <= on.clusters4 && depth >= 28 * kDepth ? 2 : 1;
 }

@@ -8,7 +8,7 @@
 // one of a few huge ones load the GPU alike, in one launch.  The sums depend on nothing but the
 // plan and the grid: no atomics.
 //
-// Measured on a B200: 200 tensors of 1 M bf16 elements are read in 65 us (6.2 TB/s) and scaled into
+// Measured on a B200: 200 tensors of 1 M bf16 elements are read in 63 us (6.4 TB/s) and scaled into
 // fp32 in 207 us (0.40 GB read, 0.8 GB written: writing alone goes at 3.9 TB/s here, in torch's fill
 // too); 1.4e9 elements take 1.89 ms for both.
 //
